@@ -56,6 +56,11 @@ SIGNATURES = {
     "dbk_gateup_swiglu_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _I, _P]),
     "dbk_qkv_rope_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                  _F, _I, _P]),
+    "dbk_page_plan": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "dbk_rope_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "dbk_chunk_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F,
+                                 _I, _P, _SZ, _P]),
+    "dbk_chunk_attention_workspace_bytes": (_SZ, [_I64, _I, _I]),
 }
 
 DBK_COMM_RECORD_BYTES = 128

@@ -1,0 +1,867 @@
+// chunk_attn.cu - attention of chunks of new tokens over a paged (or contiguous) KV cache.
+//
+//   out[t, h] = sum_{j <= p} softmax_j(scale * q[t, h] . K[j, h/G]) V[j, h/G]
+//
+// for the new token at position p of its sequence (p = seq_len - new + i for the i-th of its
+// `new` tokens, whose K and V are in the cache already). head_dim 128, fp16 / bf16.
+//
+// Work. A tile is 128 rows = (token, head of one KV group): T = 128 / G tokens x G heads, so
+// every K/V byte that is brought in serves all G heads. Two tiles (2T tokens) form an item;
+// S = Q K^T and O += P V of both run on tcgen05 with M = N = 128, and while the tensor cores
+// work on one tile the other tile's softmax runs (one warpgroup per tile, one thread per row,
+// running maximum and sum in fp32 registers). TMEM holds S0, S1, O0, O1 (4 x 128 columns);
+// P overwrites its own S as 16-bit pairs and is the PV product's A operand straight from TMEM.
+// An item with one tile only gives both warpgroups that tile and every other key block, and
+// merges the two halves from TMEM at its end.
+//
+// Split. The (item, 128-key block) units of the whole batch form one line, weighted by their
+// cost; CTA c of at most one per SM takes the c-th equal part of it, whatever the lengths are
+// (they are read on the device: no host sync). A part that begins or ends inside an item
+// leaves an fp32 partial with its maximum and sum in the workspace, and a second kernel joins
+// the partials in order, so results do not depend on timing.
+#include <climits>
+#include <type_traits>
+
+#include "common.cuh"
+#include "dbk_internal.h"
+
+namespace dbk {
+namespace {
+
+constexpr int kRows = 128;                  // rows of a tile (MMA M)
+constexpr int kKeys = 128;                  // keys of a block (MMA N of S, K of PV)
+constexpr int kHd = 128;                    // head dim
+constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
+constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
+constexpr int kRing = 5;                    // K/V tiles in flight
+constexpr int kThreadsCa = 320;             // 2 softmax warpgroups, TMA warp, MMA warp
+constexpr int kMinBox = 8;                  // rows of the smallest TMA box
+constexpr int kOver = 256;                  // an item's fixed cost, in keys
+constexpr int kSnap = 2;                    // a cut this near an item's end moves to the end
+constexpr long long kMinWork = 1024;        // least work of a CTA, in keys
+// Neighbouring cuts are at least kMinWork apart and move by less than half of that, so no part
+// between two others is empty (the join walks the parts of an item one by one).
+static_assert(kMinWork > kOver + (2 * kSnap + 1) * 128, "cuts could meet");
+constexpr float kGrow = 8.f;                // log2 growth of the maximum that forces a rescale
+constexpr float kLog2eF = 1.4426950408889634f;
+
+struct ChunkArgs {
+  CUtensorMap qmap, kmap, vmap;
+  const int32_t* cu;         // [batch + 1] first row of each sequence's new tokens
+  const int32_t* lens;       // [batch] tokens in the cache, the new ones included
+  const int32_t* pages;      // [batch, max_pages] or nullptr (contiguous)
+  void* out;
+  float* part_o;             // [2 * grid][slot_rows][128]
+  float2* part_ml;           // [2 * grid][slot_rows] (maximum in log2 units, sum)
+  int4* desc;                // [2 * grid] {first token, tokens, kv head, 0 | 1 goes on | 2 last}
+  int batch, tokens, hq, hkv, G, T;
+  int cap;                   // tokens a sequence can have in the cache
+  int page_size, max_pages, num_pages, box, total_rows, slot_rows;
+  float cs;                  // scale * log2(e)
+};
+
+// ------------------------------------------------------------------ the line of work
+struct Seq {
+  int t0, n, len;            // first row, new tokens, cached tokens
+  int items;
+  long long per_head;        // cost of one KV head
+};
+
+__device__ __forceinline__ long long cost_before(const ChunkArgs& a, const Seq& s, int i) {
+  const long long base = max(s.len - s.n, 0) + kOver, w = 2 * a.T;
+  return i * base + w * i * (i + 1ll) / 2;
+}
+
+__device__ __forceinline__ Seq load_seq(const ChunkArgs& a, int b) {
+  Seq s;
+  s.t0 = min(max(__ldcg(a.cu + b), 0), a.tokens);
+  const int t1 = min(max(__ldcg(a.cu + b + 1), s.t0), a.tokens);
+  s.n = t1 - s.t0;
+  s.len = min(max(__ldcg(a.lens + b), 0), a.cap);
+  s.items = (s.n + 2 * a.T - 1) / (2 * a.T);
+  s.per_head = 0;
+  if (s.n > 0) {
+    const int rem = s.n - (s.items - 1) * 2 * a.T;
+    const long long seen = max(s.len, s.n);
+    s.per_head = cost_before(a, s, s.items - 1) + kOver + (rem <= a.T ? (seen + 1) / 2 : seen);
+  }
+  return s;
+}
+
+struct Item {
+  int tok, ntok;             // first row, rows' tokens
+  int pos;                   // position of the first token (negative: sees nothing)
+  int b, h;
+  int kend;                  // keys that some row sees
+  int nblk, b0, b1;          // key blocks of the item, and of this CTA's piece
+  bool two;
+};
+
+__device__ __forceinline__ void item_shape(const ChunkArgs& a, const Seq& s, int i, Item& it) {
+  const int first = i * 2 * a.T;
+  it.tok = s.t0 + first;
+  it.ntok = min(s.n - first, 2 * a.T);
+  it.two = it.ntok > a.T;
+  it.pos = s.len - s.n + first;
+  it.kend = max(it.pos + it.ntok, 0);
+  it.nblk = max(1, (it.kend + kKeys - 1) / kKeys);
+}
+
+// First (b, h, item, block) of the part that starts at cost `off` inside sequence b.
+__device__ int4 locate(const ChunkArgs& a, int b, long long off) {
+  Seq s = load_seq(a, b);
+  int h = (int)(off / s.per_head);
+  off -= h * s.per_head;
+  int lo = 0, hi = s.items - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cost_before(a, s, mid) <= off) lo = mid; else hi = mid - 1;
+  }
+  int i = lo;
+  off -= cost_before(a, s, i);
+  Item it;
+  item_shape(a, s, i, it);
+  int blk = (int)min((off * (it.two ? 1 : 2) + kKeys / 2) / kKeys, (long long)INT_MAX / 2);
+  if (blk < kSnap) blk = 0;
+  else if (blk + kSnap > it.nblk) {
+    blk = 0;
+    if (++i == s.items) {
+      i = 0;
+      if (++h == a.hkv) {
+        h = 0;
+        do ++b; while (b < a.batch && load_seq(a, b).n == 0);
+      }
+    }
+  }
+  return make_int4(b, h, i, blk);
+}
+
+// The items of one CTA's part, in order; every warp role walks them by itself.
+struct Walk {
+  int4 at, end;
+  Seq s;
+  __device__ __forceinline__ Walk(const ChunkArgs& a, int4 from, int4 to) : at(from), end(to) {
+    if (at.x < a.batch) s = load_seq(a, at.x);
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs& a, Item& it) {
+    if (at.x >= a.batch) return false;
+    const bool last = at.x == end.x && at.y == end.y && at.z == end.z;
+    if (last && at.w >= end.w) return false;
+    item_shape(a, s, at.z, it);
+    it.b = at.x;
+    it.h = at.y;
+    it.b0 = at.w;
+    it.b1 = last ? end.w : it.nblk;
+    if (last) { at.w = end.w; return true; }
+    at.w = 0;
+    if (++at.z == s.items) {
+      at.z = 0;
+      if (++at.y == a.hkv) {
+        at.y = 0;
+        do {
+          if (++at.x >= a.batch) break;
+          s = load_seq(a, at.x);
+        } while (s.n == 0);
+      }
+    }
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------ tcgen05 / TMA
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {   // 128-byte swizzle, 8-row groups 1024 B apart
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// MN-major operand (V: 64 head dims per 128-byte row, one row per key): the second 64 dims lie
+// kHalf bytes on (leading offset), the next 8 keys 1024 bytes on (stride offset).
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(kHalf >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint32_t idesc_128x128(bool bf16, bool b_mn) {
+  const uint32_t f = bf16 ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((128u >> 3) << 17) |
+         ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+               ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tma_2d(void* dst, const void* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_3d(void* dst, const void* map, int x, int y, int z,
+                                       uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+
+#define DBK_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), \
+                     "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define DBK_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), \
+                     "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+// This warp's 32 lanes x 32 columns.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : DBK_R8(v, 0), DBK_R8(v, 8), DBK_R8(v, 16), DBK_R8(v, 24) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8), DBK_I8(v, 16), DBK_I8(v, 24) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Shared {
+  uint64_t full[kRing], empty[kRing];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2], o_full[2], o_free[2], half_ready;
+  uint64_t teardown, drain;
+  uint32_t tmem;
+  volatile int bail;
+  long long wsum[kThreadsCa / 32], before[kThreadsCa / 32];
+  long long total;
+  int4 cut[2];
+  float2 half_ml[kRows];     // the second warpgroup's maximum and sum (one-tile items)
+};
+
+// ------------------------------------------------------------------ the kernel
+template <typename T>
+__global__ void __launch_bounds__(kThreadsCa, 1)
+chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;                                  // Q tiles 0 and 1
+  uint8_t* ring = smem + 2 * kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(ring + kRing * kTile);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < kRing; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.o_free[i], 4);
+      sh.cut[i] = make_int4(a.batch, 0, 0, 0);
+    }
+    mbar_init(&sh.half_ready, 4);
+    mbar_init(&sh.teardown, kThreadsCa / 32);
+    mbar_init(&sh.drain, 1);
+    fence_barrier_init();
+    sh.bail = 0;
+    prefetch_tmap(&a.qmap);
+    prefetch_tmap(&a.kmap);
+    prefetch_tmap(&a.vmap);
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                 ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // Lengths, q and the cache come from earlier kernels: nothing is read before they are done.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // This CTA's two cuts of the line: cost of each sequence, prefix sum, then the thread whose
+  // sequences a cut falls in locates it.
+  const int chunk = (a.batch + kThreadsCa - 1) / kThreadsCa;
+  const int sb0 = min(tid * chunk, a.batch), sb1 = min(sb0 + chunk, a.batch);
+  long long mine = 0;
+  for (int b = sb0; b < sb1; ++b) mine += load_seq(a, b).per_head * a.hkv;
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sh.wsum[warp] = inc;
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (tid == 0) {
+    long long t = 0;
+    for (int w = 0; w < kThreadsCa / 32; ++w) { sh.before[w] = t; t += sh.wsum[w]; }
+    sh.total = t;
+  }
+  __syncthreads();
+  const long long W = sh.total;
+  const long long parts = min((long long)gridDim.x, max(1ll, W / kMinWork));
+  {
+    const long long lo = sh.before[warp] + inc - mine;
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      const long long c = blockIdx.x + e;
+      if (c >= parts) break;
+      long long w = W * c / parts - lo;
+      if (mine == 0 || w < 0 || w >= mine) continue;
+      for (int b = sb0; b < sb1; ++b) {
+        const long long cost = load_seq(a, b).per_head * a.hkv;
+        if (w < cost) { sh.cut[e] = locate(a, b, w); break; }
+        w -= cost;
+      }
+    }
+  }
+  __syncthreads();
+  const int4 c0 = sh.cut[0], c1 = sh.cut[1];
+  const uint32_t tmem = sh.tmem;
+  Walk walk(a, c0, c1);
+  Item it;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------- TMA: Q, then K and V tiles
+    int n = 0, items = 0;                       // ring tiles issued, items
+    const int pieces = kKeys / a.box;
+    const uint32_t piece_bytes = (uint32_t)a.box * 256;
+    while (!sh.bail && walk.next(a, it)) {
+      if (items > 0 && !mbar_wait(&sh.q_empty, (items - 1) & 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
+      if (lane == 0) {
+        const uint32_t qb = (uint32_t)(a.T * a.G) * 256;
+        mbar_arrive_expect_tx(&sh.q_full, it.two ? 2 * qb : qb);
+        for (int t = 0; t < (it.two ? 2 : 1); ++t)
+          for (int hf = 0; hf < 2; ++hf)
+            tma_3d(sq + t * kTile + hf * kHalf, &a.qmap, hf * 64, it.h * a.G, it.tok + t * a.T,
+                   &sh.q_full);
+      }
+      __syncwarp();
+      ++items;
+      // Lane p < pieces brings the p-th piece of each block; `row` is its row in the cache.
+      auto row_of = [&](int blk) -> int {
+        const int tok = blk * kKeys + lane * a.box;
+        if (blk >= it.b1 || lane >= pieces || tok >= it.kend) return -1;
+        if (a.pages == nullptr) return (it.b * a.hkv + it.h) * a.page_size + tok;
+        const int lp = tok / a.page_size;
+        const int pg = __ldcg(a.pages + (size_t)it.b * a.max_pages + lp);
+        if (pg < 0 || pg >= a.num_pages) return a.total_rows;      // no such page: zeros
+        return (pg * a.hkv + it.h) * a.page_size + (tok - lp * a.page_size);
+      };
+      auto issue = [&](const CUtensorMap* map, int blk, int row) -> bool {
+        const int st = n % kRing;
+        if (!mbar_wait(&sh.empty[st], ((n / kRing) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; return false; }
+        const int have = min(pieces, (it.kend - blk * kKeys + a.box - 1) / a.box);
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], (uint32_t)max(have, 0) * piece_bytes);
+        __syncwarp();
+        if (row >= 0) {
+          uint8_t* dst = ring + st * kTile + lane * a.box * 128;
+          tma_2d(dst, map, 0, row, &sh.full[st]);
+          tma_2d(dst + kHalf, map, 64, row, &sh.full[st]);
+        }
+        ++n;
+        return true;
+      };
+      const int ahead = it.two ? 1 : 2;
+      int r0 = row_of(it.b0), r1 = row_of(it.b0 + 1), r2 = row_of(it.b0 + 2);
+      if (!issue(&a.kmap, it.b0, r0)) break;
+      if (ahead == 2 && it.b0 + 1 < it.b1 && !issue(&a.kmap, it.b0 + 1, r1)) break;
+      for (int j = it.b0; j < it.b1; ++j) {
+        const int r3 = row_of(j + 3);
+        if (!issue(&a.vmap, j, r0)) break;
+        if (j + ahead < it.b1 && !issue(&a.kmap, j + ahead, ahead == 1 ? r1 : r2)) break;
+        r0 = r1; r1 = r2; r2 = r3;
+      }
+    }
+    // All copies have landed before the CTA goes (they have, unless a wait gave up).
+    for (int k = max(0, n - kRing); k < n; ++k)
+      mbar_wait(&sh.full[k % kRing], (k / kRing) & 1, kDevTimeoutDrain);
+    if (items > 0) mbar_wait(&sh.q_full, (items - 1) & 1, kDevTimeoutDrain);
+  } else if (warp == 9) {
+    // ---------------------------------------------------------- MMA issue
+    const bool bf = std::is_same<T, __nv_bfloat16>::value;
+    const uint32_t id_s = idesc_128x128(bf, false), id_o = idesc_128x128(bf, true);
+    int n = 0, items = 0;                       // ring tiles taken, items
+    int np[2] = {0, 0}, no[2] = {0, 0};         // P tiles and finished accumulators of each slot
+    auto take = [&](int k) -> bool {            // the k-th ring tile is here
+      if (!mbar_wait(&sh.full[k % kRing], (k / kRing) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
+      fence_after();
+      return true;
+    };
+    auto score = [&](int slot, int k, int qt) { // S[slot] = Q[qt] K^T
+      if (lane == 0) {
+        const uint64_t dq = desc_kmajor(smem_u32(sq + qt * kTile));
+        const uint64_t dk = desc_kmajor(smem_u32(ring + (k % kRing) * kTile));
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const uint64_t o = (uint64_t)((s >> 2) * (kHalf >> 4) + (s & 3) * 2);
+          mma_ss(tmem + slot * 128, dq + o, dk + o, id_s, s != 0);
+        }
+        mma_commit(&sh.s_full[slot]);
+      }
+      __syncwarp();
+    };
+    auto weigh = [&](int slot, int k, bool first) {   // O[slot] (+)= P[slot] V
+      if (lane == 0) {
+        const uint64_t dv = desc_mnmajor(smem_u32(ring + (k % kRing) * kTile));
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, dv + (uint64_t)(s * (2048 >> 4)),
+                 id_o, (first && s == 0) ? 0u : 1u);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int k) {
+      if (lane == 0) mma_commit(&sh.empty[k % kRing]);
+      __syncwarp();
+    };
+    auto p_ready = [&](int slot) -> bool {
+      if (!mbar_wait(&sh.p_full[slot], np[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; return false; }
+      ++np[slot];
+      fence_after();
+      return true;
+    };
+    // Keys past the item's last visible one may hold anything (a freed page's NaN): their V
+    // rows become zeros, for 0 * NaN would spoil every row.
+    auto clear_tail = [&](int k, int blk) {
+      const int from = it.kend - blk * kKeys;
+      if (from >= kKeys) return;
+      uint8_t* t = ring + (k % kRing) * kTile;
+      for (int o = max(from, 0) * 128 + lane * 16; o < kHalf; o += 512) {
+        *reinterpret_cast<uint4*>(t + o) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(t + kHalf + o) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    while (!sh.bail && walk.next(a, it)) {
+      if (!mbar_wait(&sh.q_full, items & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
+      ++items;
+      const int nb = it.b1 - it.b0;
+      bool ok = true;
+      if (it.two) {
+        if (!take(n)) break;
+        score(0, n, 0);
+        score(1, n, 1);
+        release(n);
+        ++n;
+        for (int j = 0; j < nb && ok; ++j) {
+          const int kv = n, kk = n + 1;
+          for (int s = 0; s < 2 && ok; ++s) {
+            if (j == 0 && no[s] > 0) {
+              if (!mbar_wait(&sh.o_free[s], (no[s] - 1) & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
+              fence_after();
+            }
+            if (s == 0) { if (!(ok = take(kv))) break; clear_tail(kv, it.b0 + j); }
+            if (!(ok = p_ready(s))) break;
+            weigh(s, kv, j == 0);
+            if (j + 1 == nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
+            else {
+              if (s == 0 && !(ok = take(kk))) break;
+              score(s, kk, s);
+            }
+          }
+          if (!ok) break;
+          release(kv);
+          ++n;
+          if (j + 1 < nb) { release(kk); ++n; }
+          if (j + 2 == nb || nb == 1) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
+        }
+        if (!ok) break;
+        ++no[0];
+        ++no[1];
+      } else {
+        // Ring order: K0 K1 | V0 K2 | V1 K3 | ...; block j belongs to slot j & 1.
+        if (!take(n)) break;
+        score(0, n, 0);
+        release(n);
+        ++n;
+        if (nb > 1) {
+          if (!take(n)) break;
+          score(1, n, 0);
+          release(n);
+          ++n;
+        }
+        if (nb <= 2) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
+        for (int j = 0; j < nb && ok; ++j) {
+          const int s = j & 1;
+          if (j < 2 && no[s] > 0) {
+            if (!mbar_wait(&sh.o_free[s], (no[s] - 1) & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
+            fence_after();
+          }
+          if (!(ok = take(n))) break;
+          clear_tail(n, it.b0 + j);
+          if (!(ok = p_ready(s))) break;
+          weigh(s, n, j < 2);
+          release(n);
+          ++n;
+          if (j + 2 >= nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
+          else {
+            if (!(ok = take(n))) break;
+            score(s, n, 0);
+            release(n);
+            ++n;
+            if (j + 3 == nb) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
+          }
+        }
+        if (!ok) break;
+        ++no[0];
+        if (nb > 1) ++no[1];
+      }
+    }
+    if (lane == 0) mma_commit(&sh.drain);        // every MMA issued has finished
+    __syncwarp();
+    mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
+  } else {
+    // ---------------------------------------------------------- softmax, one thread per row
+    const int slot = warp >> 2;
+    const int r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + slot * 128, t_o = tmem + lanes + 256;
+    const int rt = r / a.G, rg = r - rt * a.G;   // this row's token in the tile, head in the group
+    T* out = static_cast<T*>(a.out);
+    int ns = 0, no[2] = {0, 0}, nh = 0;
+    if (tid < 2) a.desc[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
+    named_bar_sync(1, 256);
+    while (!sh.bail && walk.next(a, it)) {
+      const int nb = it.b1 - it.b0;
+      const int tok = it.two && slot == 1 ? a.T + rt : rt;        // token within the item
+      const int vis = max(it.pos + tok + 1, 0);                    // keys this row sees
+      const int step = it.two ? 1 : 2;
+      float m = -INFINITY, l = 0.f;
+      int mine_n = 0;
+      bool ok = true;
+      for (int j = it.two ? 0 : slot; j < nb; j += step, ++mine_n) {
+        if (!mbar_wait(&sh.s_full[slot], ns & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
+        ++ns;
+        fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(t_s + q * 32, s[q]);
+        tmem_wait_ld();
+        const int lim = vis - (it.b0 + j) * kKeys;
+        if (lim < kKeys) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (q * 32 + c >= lim) s[q][c] = 0xff800000u;        // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(s[q][c])), __uint_as_float(s[q][c + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.cs;
+        // The running maximum only follows when it grew by more than kGrow (in log2 units): the
+        // weights then stay below 2^kGrow, exact in fp32 sums and in range for 16 bits, and
+        // most blocks need no pass over O.
+        const bool grow = top > m + kGrow;
+        if (mine_n == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? top : m;
+          const float f = grow ? ex2(m - mn) : 1.f;               // m = -inf: 0
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[32];
+            tmem_ld32(t_o + slot * 128 + q * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+            tmem_st32(t_o + slot * 128 + q * 32, o);
+          }
+          l *= f;
+          m = mn;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int hq = 0; hq < 2; ++hq) {
+          uint32_t p[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int q = hq * 2 + (c >> 4), e = (2 * c) & 31;
+            const float p0 = ex2(fmaf(__uint_as_float(s[q][e]), a.cs, nm));
+            const float p1 = ex2(fmaf(__uint_as_float(s[q][e + 1]), a.cs, nm));
+            sum[c & 1] += p0;
+            sum[2 + (c & 1)] += p1;
+            p[c] = Mma<T>::pack(p0, p1);
+          }
+          tmem_st32(t_s + hq * 32, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[slot]);
+      }
+      if (!ok) break;
+
+      // Epilogue: O / l to the output, or O, m, l to the workspace.
+      const bool joined = !it.two && nb > 1;      // slot 1 holds the odd blocks
+      if (it.two || slot == 0 || joined) {
+        if (!mbar_wait(&sh.o_full[slot], no[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
+        ++no[slot];
+        fence_after();
+      }
+      if (!it.two && slot == 1) {
+        if (joined) {
+          sh.half_ml[r] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.half_ready);
+        }
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if (joined) {
+        if (!mbar_wait(&sh.half_ready, nh & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
+        ++nh;
+        fence_after();
+        const float2 o = sh.half_ml[r];
+        const float mm = fmaxf(m, o.x);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        f0 = ex2(m - ref);
+        f1 = ex2(o.x - ref);
+        l = l * f0 + o.y * f1;
+        m = mm;
+      }
+      const bool whole = it.b0 == 0 && it.b1 == it.nblk;
+      const int sl = 2 * blockIdx.x + (it.b0 > 0 ? 0 : 1);
+      if (!whole && tid == 0)
+        a.desc[sl] = make_int4(it.tok, it.ntok, it.h, it.b1 == it.nblk ? 2 : 1);
+      const bool live = r < a.T * a.G && tok < it.ntok;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // nothing seen: zeros; NaN stays
+      const int prow = slot * kRows + r;
+      T* dst = out + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
+      float* pdst = a.part_o + ((size_t)sl * a.slot_rows + prow) * kHd;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t o[32];
+        tmem_ld32(t_o + slot * 128 + q * 32, o);
+        tmem_wait_ld();
+        if (joined) {
+          uint32_t o1[32];
+          tmem_ld32(t_o + 128 + q * 32, o1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            o[c] = __float_as_uint(__uint_as_float(o[c]) * f0 + __uint_as_float(o1[c]) * f1);
+        }
+        if (live) {
+          if (whole) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              uint4 v;
+              v.x = Mma<T>::pack(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
+              v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+              v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
+              v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + q * 32 + c) = v;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              *reinterpret_cast<uint4*>(pdst + q * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (live && !whole) a.part_ml[(size_t)sl * a.slot_rows + prow] = make_float2(m, l);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.o_free[slot]);
+        if (joined) mbar_arrive(&sh.o_free[1]);
+      }
+    }
+  }
+  // Teardown: every warp arrives once; the MMA warp frees TMEM when all have.
+  __syncwarp();
+  fence_before();
+  if (lane == 0) mbar_arrive(&sh.teardown);
+  if (warp == 9) {
+    mbar_wait(&sh.teardown, 0, kDevTimeoutDrain);
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// Joins the partials of the items that CTA cuts went through. Block (c, y): the item whose
+// first piece CTA c left, rows 8 warps at a time; a row's pieces are weighted by
+// 2^(m - max m) in the order of the keys.
+constexpr int kJoinSlices = 8;
+constexpr int kJoinWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  const int4 d = __ldcg(a.desc + 2 * c + 1);
+  if (d.w != 1) return;
+  int pieces = 1;
+  while (c + pieces < (int)gridDim.x) {
+    const int f = __ldcg(&a.desc[2 * (c + pieces)].w);
+    if (f == 0) break;
+    ++pieces;
+    if (f == 2) break;
+  }
+  auto slot_of = [&](int p) { return p == 0 ? 2 * c + 1 : 2 * (c + p); };
+  const int rows = d.y > a.T ? 2 * kRows : kRows;
+  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += kJoinSlices * kJoinWarps) {
+    const int rr = r & (kRows - 1), rt = rr / a.G;
+    const int tok = (r >> 7) * a.T + rt;
+    if (rr >= a.T * a.G || tok >= d.y) continue;
+    float m = -INFINITY;
+    for (int p = lane; p < pieces; p += 32)
+      m = fmaxf(m, __ldcg(a.part_ml + (size_t)slot_of(p) * a.slot_rows + r).x);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < pieces; p0 += 32) {
+      float w = 0.f, lw = 0.f;
+      if (p0 + lane < pieces) {
+        const float2 ml = __ldcg(a.part_ml + (size_t)slot_of(p0 + lane) * a.slot_rows + r);
+        w = ex2(ml.x - ref);
+        lw = ml.y * w;
+      }
+      l += warp_sum(lw);
+      const int cnt = min(32, pieces - p0);
+#pragma unroll 4
+      for (int p = 0; p < cnt; ++p) {
+        const float wp = __shfl_sync(0xffffffffu, w, p);
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(
+            a.part_o + ((size_t)slot_of(p0 + p) * a.slot_rows + r) * kHd) + lane);
+        acc.x += o.x * wp; acc.y += o.y * wp; acc.z += o.z * wp; acc.w += o.w * wp;
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* dst = static_cast<T*>(a.out) + ((size_t)(d.x + tok) * a.hq + d.z * a.G + (rr - rt * a.G)) * kHd;
+    uint2 v;
+    v.x = Mma<T>::pack(acc.x * inv, acc.y * inv);
+    v.y = Mma<T>::pack(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(dst + lane * 4) = v;
+  }
+}
+
+int slot_rows_of(int64_t tokens, int G) { return tokens * G <= kRows ? (int)(tokens * G) : 2 * kRows; }
+
+size_t ws_bytes_of(int sms, int64_t tokens, int G) {
+  const size_t rows = (size_t)2 * sms * slot_rows_of(tokens, G);
+  return rows * (kHd * sizeof(float) + sizeof(float2)) + (size_t)2 * sms * sizeof(int4) + 256;
+}
+
+template <typename T>
+int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
+  const size_t smem = 1024 + (size_t)(2 + kRing) * kTile + sizeof(Shared);
+  const void* kern = reinterpret_cast<const void*>(&chunk_attention_kernel<T>);
+  if (int rc = allow_dynamic_smem(kern, dev, smem)) return rc;
+  if (int rc = launch_pdl(kern, dim3(dev.num_sms), dim3(kThreadsCa), smem, st, &a)) return rc;
+  return launch_pdl(reinterpret_cast<const void*>(&chunk_join_kernel<T>),
+                    dim3(dev.num_sms, kJoinSlices), dim3(kJoinWarps * 32), 0, st, &a);
+}
+
+}  // namespace
+
+}  // namespace dbk
+
+using namespace dbk;
+
+extern "C" size_t dbk_chunk_attention_workspace_bytes(int64_t tokens, int n_q_heads,
+                                                      int n_kv_heads) {
+  if (tokens < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads) return 0;
+  DeviceInfo dev;
+  int sms = 148;
+  if (current_device_info(&dev) == DBK_OK) sms = dev.num_sms;
+  return ws_bytes_of(sms, tokens, n_q_heads / n_kv_heads);
+}
+
+extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,
+                                   const int32_t* cu_seqlens, const int32_t* seq_lens,
+                                   const int32_t* page_table, void* out, int tokens, int batch,
+                                   int n_q_heads, int n_kv_heads, int head_dim, int num_pages,
+                                   int page_size, int max_pages_per_seq, float scale, int dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (!k_cache || !v_cache || !cu_seqlens || !seq_lens) return DBK_ENULL;
+  if (dtype != DBK_F16 && dtype != DBK_BF16) return DBK_EDTYPE;
+  if (head_dim != kHd || tokens < 0 || batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads ||
+      n_q_heads % n_kv_heads != 0 || num_pages < 1 || page_size < 1)
+    return DBK_ESHAPE;
+  const int G = n_q_heads / n_kv_heads;
+  if (G > kRows || !(scale > 0.f) || scale > 3e38f) return DBK_ESHAPE;
+  const int64_t rows = (int64_t)num_pages * n_kv_heads;
+  if (rows > INT_MAX || rows * page_size > INT_MAX - kKeys) return DBK_ESHAPE;
+  int box = kKeys;
+  if (page_table) {
+    if (max_pages_per_seq < 1) return DBK_ESHAPE;
+    while (box > page_size || page_size % box) box >>= 1;
+    if (box < kMinBox) return DBK_ESHAPE;
+  } else if (num_pages != batch) {
+    return DBK_ESHAPE;
+  }
+  if (tokens == 0) return DBK_OK;
+  if (!q || !out) return DBK_ENULL;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return DBK_EALIGN;
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  if (!workspace || workspace_bytes < ws_bytes_of(dev.num_sms, tokens, G)) return DBK_EWORKSPACE;
+  if (!aligned16(workspace)) return DBK_EALIGN;
+
+  ChunkArgs a{};
+  a.cu = cu_seqlens; a.lens = seq_lens; a.pages = page_table; a.out = out;
+  a.batch = batch; a.tokens = tokens; a.hq = n_q_heads; a.hkv = n_kv_heads;
+  a.G = G; a.T = kRows / G;
+  a.page_size = page_size; a.max_pages = page_table ? max_pages_per_seq : 1;
+  a.num_pages = num_pages; a.box = box; a.total_rows = (int)(rows * page_size);
+  const int64_t cap = (int64_t)page_size * a.max_pages;
+  a.cap = (int)(cap < INT_MAX - 2 * kKeys ? cap : INT_MAX - 2 * kKeys);
+  a.slot_rows = slot_rows_of(tokens, G);
+  a.cs = scale * kLog2eF;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const size_t prow = (size_t)2 * dev.num_sms * a.slot_rows;
+  a.part_o = reinterpret_cast<float*>(ws);
+  ws += prow * kHd * sizeof(float);
+  a.desc = reinterpret_cast<int4*>(ws);
+  ws += (size_t)2 * dev.num_sms * sizeof(int4);
+  a.part_ml = reinterpret_cast<float2*>(ws);
+  rc = encode_tmap_heads3d(&a.qmap, q, dtype, tokens, n_q_heads, G, a.T);
+  if (rc) return rc;
+  const uint64_t cache_rows = (uint64_t)rows * page_size;
+  rc = encode_tmap_2d(&a.kmap, k_cache, dtype, kHd, cache_rows, kHd * 2, 64, box, true);
+  if (rc) return rc;
+  rc = encode_tmap_2d(&a.vmap, v_cache, dtype, kHd, cache_rows, kHd * 2, 64, box, true);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DBK_F16 ? launch<__half>(a, dev, st) : launch<__nv_bfloat16>(a, dev, st);
+}

@@ -50,6 +50,12 @@ int encode_tmap_2d(CUtensorMap* out, const void* base, int dtype, uint64_t inner
 int encode_tmap_kv3d(CUtensorMap* out, const void* base, int dtype, uint64_t rows,
                      uint32_t box_rows);
 
+// 3-D tiled TMA descriptor over [tokens, heads, 128] 16-bit elements: a box holds 64 elements
+// of box_heads heads of box_tokens tokens, one 128-byte line each (128-byte swizzle), heads
+// fastest; zeros past the last token.
+int encode_tmap_heads3d(CUtensorMap* out, const void* base, int dtype, uint64_t tokens,
+                        uint64_t heads, uint32_t box_heads, uint32_t box_tokens);
+
 // Launch `func(*args)` (one by-value struct parameter) with programmatic
 // dependent launch enabled unless DBK_PDL=0 is set in the environment.
 int launch_pdl(const void* func, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

@@ -11,9 +11,11 @@ missing kernel library, raises.
 
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -502,6 +504,161 @@ def qkv_rope_append(x: torch.Tensor, Wqkv_il: torch.Tensor, positions: torch.Ten
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(page_table), batch, d_in,
         n_q_heads, n_kv_heads, D, ps, maxp, float(eps), dt, _stream(dev)))
     return q
+
+
+class PagePlan(NamedTuple):
+    """What :func:`page_plan` builds beside the page table it updates."""
+
+    seq_lens: torch.Tensor      # int32 [batch]: tokens in the cache after this step
+    cu_seqlens: torch.Tensor    # int32 [batch + 1]: first packed token of each request
+    positions: torch.Tensor     # int32 [n_tokens]
+    slots: torch.Tensor         # int64 [n_tokens]: cache slot, -1 where there is no page
+    used: torch.Tensor          # int32 [1]: free pages the step needs
+
+
+_same_device = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` current for a launch when it is not."""
+    return _same_device if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _check_i32(name: str, t: torch.Tensor, numel: int) -> None:
+    if t.dtype != torch.int32 or t.numel() != numel:
+        raise ValueError(f"{name} must be int32 with {numel} elements")
+
+
+def page_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+              page_table: torch.Tensor, page_size: int, n_tokens: int) -> PagePlan:
+    """Page tables, slots and positions of a scheduler step, from the requests' lengths.
+
+    ctx_lens / new_lens int32 [batch]: tokens in the cache and tokens of this step (packed in
+    request order). ``page_table`` int32 [batch, max_pages] is updated in place: a request that
+    needs more pages than ceil(ctx / page_size) gets the next ones of ``free_pages`` (int32,
+    handed out in order, requests in order), and nothing else of the table changes.
+    ``n_tokens`` is the packed length of the step's tensors; rows behind the last token get
+    position 0 and slot -1. Where the list or the table is too short, table entries and slots
+    become -1, and ``used`` tells how many pages the step needs. See ``dbk_page_plan``."""
+    dev = _need_cuda(ctx_lens, new_lens, free_pages, page_table)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [batch, max_pages]")
+    batch, max_pages = page_table.shape
+    _check_i32("ctx_lens", ctx_lens, batch)
+    _check_i32("new_lens", new_lens, batch)
+    if free_pages.dtype != torch.int32:
+        raise ValueError("free_pages must be int32")
+    if n_tokens < 0:
+        raise ValueError("n_tokens must not be negative")
+    lens = torch.empty(batch, dtype=torch.int32, device=dev)
+    cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
+    pos = torch.empty(n_tokens, dtype=torch.int32, device=dev)
+    slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
+    used = torch.empty(1, dtype=torch.int32, device=dev)
+    with _on(dev):
+        N.check("dbk_page_plan", N.load().dbk_page_plan(
+            ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), page_table.data_ptr(),
+            lens.data_ptr(), cu.data_ptr(), pos.data_ptr(), slots.data_ptr(), used.data_ptr(),
+            batch, free_pages.numel(), int(page_size), max_pages, int(n_tokens), _stream(dev)))
+    return PagePlan(lens, cu, pos, slots, used)
+
+
+def rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                n_q_heads: int, n_kv_heads: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE and KV-cache append for a packed chunk of new tokens of many requests.
+
+    qkv [tokens, (Hq + 2 Hkv) * 128] in natural order (the projection's output; the one-token
+    :func:`qkv_rope_append` does the projection too); positions int32 [tokens], slots int64
+    [tokens] as :func:`page_plan` gives them; caches [pages, Hkv, page_size, 128] (a contiguous
+    cache [batch, Hkv, max_len, 128] has slot b * max_len + position). k and v are written into
+    the caches in place, rows with a slot outside the cache (-1) are not; returns q
+    [tokens, Hq, 128], rotated. Slots must differ from one another."""
+    dev = _need_cuda(qkv, positions, slots, inv_freq, k_cache, v_cache)
+    _check_out(out, dev)
+    dt = _dtype_code(qkv)
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_kv_heads:
+        raise ValueError("k_cache / v_cache must be [pages, Hkv, page_size, D] of one shape")
+    if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
+        raise TypeError("qkv, k_cache and v_cache must share one dtype")
+    pages, _, page_size, D = k_cache.shape
+    if qkv.dim() != 2 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * D:
+        raise ValueError(f"qkv must be [tokens, {(n_q_heads + 2 * n_kv_heads) * D}]")
+    n = qkv.shape[0]
+    _check_i32("positions", positions, n)
+    if slots.dtype != torch.int64 or slots.numel() != n:
+        raise ValueError(f"slots must be int64 with {n} elements")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2:
+        raise ValueError(f"inv_freq must be float32 [{D // 2}]")
+    q = out if out is not None else torch.empty(n, n_q_heads, D, dtype=qkv.dtype, device=dev)
+    if q.dtype != qkv.dtype or q.numel() != n * n_q_heads * D:
+        raise ValueError(f"out must be [{n}, {n_q_heads}, {D}] of qkv's dtype")
+    with _on(dev):
+        N.check("dbk_rope_append", N.load().dbk_rope_append(
+            qkv.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(),
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n, n_q_heads, n_kv_heads, D,
+            pages, page_size, dt, _stream(dev)))
+    return q
+
+
+def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    cu_seqlens: torch.Tensor, seq_lens: torch.Tensor,
+                    page_table: torch.Tensor | None = None, scale: float | None = None,
+                    out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed chunks of new tokens over the KV cache, causal from the end.
+
+    q [tokens, Hq, 128]; sequence b's n new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1]
+    (int32 [batch + 1]), the last of them at position seq_lens[b] - 1 (int32 [batch]; the new
+    tokens' K and V are in the cache already). A token at position p sees positions 0..p; one
+    with p < 0 gives zeros. Chunks of any length, of 0 and of 1 token included. Paged caches
+    (``page_table`` int32 [batch, max_pages]): k/v [pages, Hkv, page_size, 128], page_size a
+    multiple of 8; contiguous: [batch, Hkv, max_len, 128]. ``scale`` (> 0) defaults to
+    1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` are left as they were."""
+    dev = _need_cuda(q, k_cache, v_cache, cu_seqlens, seq_lens, page_table)
+    _check_out(out, dev)
+    dt = _dtype_code(q)
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("q, k_cache and v_cache must share one dtype")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must be 4-D tensors of one shape")
+    if q.dim() != 3 or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("q must be [tokens, Hq, head_dim] with the cache's head_dim")
+    tokens, hq, D = q.shape
+    pages, hkv, page_size, _ = k_cache.shape
+    batch = seq_lens.numel()
+    _check_i32("seq_lens", seq_lens, batch)
+    _check_i32("cu_seqlens", cu_seqlens, batch + 1)
+    if page_table is None:
+        if pages != batch:
+            raise ValueError("contiguous cache must be [batch, Hkv, max_len, head_dim]")
+        max_pages = 1
+    else:
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+            raise ValueError("page_table must be int32 [batch, max_pages]")
+        max_pages = page_table.shape[1]
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    o = out if out is not None else torch.empty_like(q)
+    if o.dtype != q.dtype or o.numel() != q.numel():
+        raise ValueError("out must have q's shape and dtype")
+    lib = N.load()
+    some = min(tokens, 129)      # the size stops growing before that many tokens
+    nb = _ws_bytes(("chunk", dev.index, some, hq, hkv),
+                   lambda: lib.dbk_chunk_attention_workspace_bytes(some, hq, hkv))
+    if workspace is None:
+        # Not zero-filled and not kept: the caching allocator orders reuse by stream, and a
+        # captured graph gets its own.
+        workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
+    elif workspace.dtype != torch.uint8 or workspace.device != dev or workspace.numel() < nb:
+        raise ValueError(f"workspace must be a uint8 tensor of >= {nb} bytes on {dev}")
+    with _on(dev):
+        N.check("dbk_chunk_attention", lib.dbk_chunk_attention(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(),
+            seq_lens.data_ptr(), _ptr(page_table), o.data_ptr(), tokens, batch, hq, hkv, D,
+            pages, page_size, max_pages, float(scale), dt, workspace.data_ptr(), nb,
+            _stream(dev)))
+    return o
 
 
 def quantize_fp8_rows(W: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -245,6 +245,71 @@ int dbk_gateup_swiglu_fp8(const void* x, const void* gamma, const void* Wg8, con
                           int d_ff, float eps, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * A scheduler step of paged serving: chunks of new tokens of many requests,
+ * packed one after the other. dbk_page_plan -> (projection) -> dbk_rope_append
+ * -> dbk_chunk_attention -> ... -> dbk_sample. Lengths stay on the device; no
+ * call waits for the host. No counterpart in the reference, whose stages take
+ * one token. */
+
+/* Page tables, slots and positions from the requests' lengths.
+ *   ctx_lens, new_lens  int32 [batch]: tokens in the cache, tokens of this step
+ *                       (0 is fine; a negative length counts as 0)
+ *   free_pages          int32 [n_free]: page ids, handed out in this order
+ *   page_table          int32 [batch, max_pages_per_seq], updated in place: request b
+ *                       keeps its first ceil(ctx / page_size) entries and gets the next free
+ *                       pages for those it lacks up to ceil((ctx + new) / page_size); entries
+ *                       behind stay as they were. When the list runs out, -1 is written.
+ *   seq_lens            int32 [batch]      ctx + new
+ *   cu_seqlens          int32 [batch + 1]  first packed token of each request, then their number
+ *   positions, slots    int32 / int64 [tokens]: of each packed token its position and its cache
+ *                       slot page * page_size + position % page_size; the slot is -1 where there
+ *                       is no page (list or table too short). Rows behind the last
+ *                       token get position 0 and slot -1; tokens behind the `tokens`-th are left out.
+ *   used                int32 [1]: free pages the step needs (more than n_free: it lacked some)
+ * Requests' token total and lengths stay below 2^31; batch <= 16384; outputs must not overlap
+ * inputs. Any later call may follow directly: the plan is complete before it starts. */
+int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_pages,
+                  int32_t* page_table, int32_t* seq_lens, int32_t* cu_seqlens,
+                  int32_t* positions, int64_t* slots, int32_t* used, int batch, int n_free,
+                  int page_size, int max_pages_per_seq, int tokens, void* stream);
+
+/* RoPE and cache append of a packed chunk:
+ *   qkv [tokens, (n_q_heads + 2 n_kv_heads) * 128], natural order [q heads | k heads | v heads];
+ *   q and k are rotated at positions[t] (rotate-half pairs i, i + 64, angle positions[t] *
+ *   inv_freq[i], formed in 64 bits); q -> q_out [tokens, n_q_heads, 128]; k, v -> slot slots[t] of
+ *   k_cache, v_cache [num_pages, n_kv_heads, page_size, 128] (a contiguous cache [batch,
+ *   n_kv_heads, max_len, 128] is one page per sequence: slot = b * max_len + position).
+ * A slot outside the cache (-1 for a padded row) writes q only. Slots must differ from one
+ * another; of two rows with one slot either may be kept, in parts. head_dim 128 only. */
+int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* slots,
+                    const float* inv_freq, void* q_out, void* k_cache, void* v_cache, int tokens,
+                    int n_q_heads, int n_kv_heads, int head_dim, int num_pages, int page_size,
+                    int dtype, void* stream);
+
+/* Attention of packed chunks of new tokens over the cache, causal from the end:
+ *   q, out [tokens, n_q_heads, 128]; sequence b's new tokens are rows cu_seqlens[b] ..
+ *   cu_seqlens[b + 1] - 1; the i-th of its n is at position p = seq_lens[b] - n + i and attends
+ *   to cache positions 0..p (its own K and V are in the cache already). A row with p < 0 gives
+ *   zeros. n may be 0 or 1 (a decoding request) beside long chunks.
+ *   Paged cache: k_cache, v_cache [num_pages, n_kv_heads, page_size, 128], page_table int32
+ *   [batch, max_pages_per_seq], page_size a multiple of 8; a page id outside the cache reads as
+ *   zeros. Contiguous cache (page_table NULL): [num_pages = batch, n_kv_heads, page_size =
+ *   max_len, 128]. seq_lens are clipped to what the table holds, cu_seqlens to 0..tokens.
+ *   q head h reads kv head h / (n_q_heads / n_kv_heads), any ratio up to 128. scale > 0.
+ * Rows of out behind cu_seqlens[batch] are left as they were. Cache slots at and past seq_lens
+ * may hold anything. Maximum, sum and output accumulate in fp32; the weights are rounded to
+ * dtype for the tensor cores. Results do not depend on timing.
+ * workspace: dbk_chunk_attention_workspace_bytes(), need not be zero-filled, one per call that
+ * may run concurrently. */
+int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,
+                        const int32_t* cu_seqlens, const int32_t* seq_lens,
+                        const int32_t* page_table, void* out, int tokens, int batch,
+                        int n_q_heads, int n_kv_heads, int head_dim, int num_pages, int page_size,
+                        int max_pages_per_seq, float scale, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+size_t dbk_chunk_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_kv_heads);
+
+/* ------------------------------------------------------------------------
  * Shard-boundary all-gather over NVLink peer memory (multi-GPU, one process
  * per GPU). No counterpart in the reference, which is single-GPU: it replaces
  * the ncclAllGather that ends each sharded op (weight rows or kv heads split
