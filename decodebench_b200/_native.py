@@ -12,7 +12,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libdbk.so"
 
-DBK_F16, DBK_BF16 = 0, 1
+DBK_F16, DBK_BF16, DBK_F32 = 0, 1, 2
 DBK_ESHAPE = -2
 DBK_OP_RMSNORM_GEMV, DBK_OP_GATEUP_SWIGLU, DBK_OP_GEMV = 0, 1, 2
 
@@ -61,6 +61,7 @@ SIGNATURES = {
     "dbk_chunk_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F,
                                  _I, _P, _SZ, _P]),
     "dbk_chunk_attention_workspace_bytes": (_SZ, [_I64, _I, _I]),
+    "dbk_sample": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _I, _F, _F, _I, _P]),
 }
 
 DBK_COMM_RECORD_BYTES = 128

@@ -167,21 +167,35 @@ int encode_tmap_heads3d(CUtensorMap* out, const void* base, int dtype, uint64_t 
   return r == CUDA_SUCCESS ? DBK_OK : DBK_ESHAPE;
 }
 
-int launch_pdl(const void* func, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-               void* args) {
+int launch_pdl_cluster(const void* func, dim3 grid, dim3 block, int cluster, size_t smem,
+                       cudaStream_t stream, void* args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = n;
   void* params[1] = {args};
   cudaError_t e = cudaLaunchKernelExC(&cfg, func, params);
   return e == cudaSuccess ? DBK_OK : (int)e;
+}
+
+int launch_pdl(const void* func, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+               void* args) {
+  return launch_pdl_cluster(func, grid, block, 1, smem, stream, args);
 }
 
 }  // namespace dbk

@@ -60,6 +60,9 @@ int encode_tmap_heads3d(CUtensorMap* out, const void* base, int dtype, uint64_t 
 // dependent launch enabled unless DBK_PDL=0 is set in the environment.
 int launch_pdl(const void* func, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                void* args);
+// The same with thread-block clusters of `cluster` CTAs along x (1..8).
+int launch_pdl_cluster(const void* func, dim3 grid, dim3 block, int cluster, size_t smem,
+                       cudaStream_t stream, void* args);
 
 }  // namespace dbk
 

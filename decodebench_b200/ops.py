@@ -661,6 +661,55 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return o
 
 
+def _per_row(name: str, v, dtype: torch.dtype, batch: int, off):
+    """(tensor or None, value for all rows) of a sampling parameter."""
+    if v is None:
+        return None, off
+    if isinstance(v, torch.Tensor):
+        if v.dtype != dtype or v.numel() != batch:
+            raise ValueError(f"{name} must be a number or a {dtype} tensor with {batch} elements")
+        return v, off
+    if v != v:
+        raise ValueError(f"{name} must not be NaN")
+    return None, v
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=None, top_p=None,
+           min_p=None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The next token of each row of logits [batch, vocab] (fp32, fp16 or bf16): int64 [batch].
+
+    Weights exp((x - max) / temperature); ``top_k`` keeps the first k logits (larger first, of
+    equal ones the lower index), ``top_p`` of those the shortest prefix with at least top_p of
+    their weight, ``min_p`` of those the ones with at least min_p of the largest weight. The
+    token is the first index whose running sum of kept weights exceeds uniforms[b] (fp32, in
+    [0, 1)) times their sum; temperature <= 0 takes the largest logit. Each parameter is a
+    number or a tensor [batch] (fp32, ``top_k`` int32; None, top_k <= 0, top_p >= 1 and
+    min_p <= 0 are off). NaN counts as -inf; a row of nothing but -inf gives -1."""
+    dev = _need_cuda(logits, uniforms, *(t for t in (temperature, top_k, top_p, min_p)
+                                         if isinstance(t, torch.Tensor)))
+    if logits.dim() != 2:
+        raise ValueError("logits must be [batch, vocab]")
+    dt = N.DBK_F32 if logits.dtype == torch.float32 else _dtype_code(logits)
+    batch, vocab = logits.shape
+    if uniforms.dtype != torch.float32 or uniforms.numel() != batch:
+        raise ValueError(f"uniforms must be float32 with {batch} elements")
+    f32 = torch.float32
+    t, t_all = _per_row("temperature", temperature, f32, batch, 1.0)
+    k, k_all = _per_row("top_k", top_k, torch.int32, batch, 0)
+    p, p_all = _per_row("top_p", top_p, f32, batch, 1.0)
+    m, m_all = _per_row("min_p", min_p, f32, batch, 0.0)
+    o = out if out is not None else torch.empty(batch, dtype=torch.int64, device=dev)
+    if o.dtype != torch.int64 or o.numel() != batch:
+        raise ValueError(f"out must be int64 with {batch} elements")
+    _check_out(out, dev)
+    with _on(dev):
+        N.check("dbk_sample", N.load().dbk_sample(
+            logits.data_ptr(), uniforms.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m),
+            o.data_ptr(), batch, vocab, float(t_all), max(0, min(int(k_all), 2 ** 31 - 1)),
+            float(p_all), float(m_all), dt, _stream(dev)))
+    return o
+
+
 def quantize_fp8_rows(W: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-row e4m3 quantisation for the fp8 GEMVs: returns (W8, scale) with
     W ~= scale[:, None] * W8.float(); scale = amax(|row|) / 448 (fp32)."""

@@ -30,6 +30,7 @@ extern "C" {
 
 /* Element type of activations, weights, caches and outputs. */
 typedef enum { DBK_F16 = 0, DBK_BF16 = 1 } dbk_dtype;
+#define DBK_F32 2             /* logits of dbk_sample only */
 
 /* Argument errors (negative). Positive values are cudaError_t. */
 #define DBK_OK 0
@@ -308,6 +309,22 @@ int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,
                         int max_pages_per_seq, float scale, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream);
 size_t dbk_chunk_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_kv_heads);
+
+/* The next token of each row of logits [batch, vocab] (dtype DBK_F16, DBK_BF16 or DBK_F32;
+ * vocab <= 2^20) from one random number per row, uniforms [batch] in [0, 1):
+ *   w_i = exp((x_i - max) / temperature); order: larger logit first, then lower index.
+ *   top_k > 0 keeps the first top_k of the order; top_p < 1 keeps of those the shortest prefix
+ *   whose weights reach top_p of their sum (at least one); min_p > 0 keeps of those w_i >= min_p.
+ *   tokens[b] (int64) = the first index whose running sum of kept weights, in index order,
+ *   exceeds uniforms[b] * their sum. temperature <= 0: the first of the order.
+ * temperature, top_k, top_p, min_p: device arrays [batch], or NULL for the value given for all
+ * rows (top_k <= 0, top_p >= 1, min_p <= 0: off). NaN logits count as -inf; a row with
+ * nothing but -inf gives -1; logits of +inf share the draw alike. min_p above 1 keeps what
+ * min_p = 1 keeps. Sums are 64-bit and do not depend on timing. */
+int dbk_sample(const void* logits, const float* uniforms, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens,
+               int batch, int vocab, float temperature_all, int top_k_all, float top_p_all,
+               float min_p_all, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Shard-boundary all-gather over NVLink peer memory (multi-GPU, one process

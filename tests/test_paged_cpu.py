@@ -84,3 +84,20 @@ def test_ops_refuse_cpu_tensors():
                         z(2, 1, 16, 128), 2, 1)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ops.chunk_attention(z(3, 2, 128), z(2, 1, 16, 128), z(2, 1, 16, 128), i(2), i(1), i(1, 2))
+
+
+def sample(**kw):
+    a = dict(x=16, u=16, t=None, k=None, p=None, mp=None, out=16, batch=2, vocab=100, temp=1.0,
+             top_k=0, top_p=1.0, min_p=0.0, dt=2)
+    a.update(kw)
+    return N.load().dbk_sample(*[a[k] for k in ("x", "u", "t", "k", "p", "mp", "out", "batch", "vocab",
+                                                "temp", "top_k", "top_p", "min_p", "dt")], None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(x=None), ENULL), (dict(u=None), ENULL), (dict(out=None), ENULL), (dict(vocab=0), ESHAPE),
+    (dict(vocab=(1 << 20) + 1), ESHAPE), (dict(batch=-1), ESHAPE), (dict(dt=5), EDTYPE),
+    (dict(x=4), EALIGN), (dict(temp=float("nan")), ESHAPE), (dict(top_p=float("nan")), ESHAPE),
+    (dict(batch=0, x=None), 0)])
+def test_sample_refusals(kw, want):
+    assert sample(**kw) == want
