@@ -34,7 +34,12 @@ constexpr int kHd = 128;                    // head dim
 constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
 constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
 constexpr int kRing = 5;                    // K/V tiles in flight
-constexpr int kThreadsCa = 320;             // 2 softmax warpgroups, TMA warp, MMA warp
+constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA warp, MMA warp, 2 idle
+// Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup gives
+// up all but 40, which lets a softmax thread hold its row of S (128 values) without spilling:
+// 256 x 232 + 128 x 40 = 384 x 168.
+constexpr int kRegsSoftmax = 232, kRegsOther = 40;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
 constexpr int kSnap = 2;                    // a cut this near an item's end moves to the end
@@ -43,6 +48,7 @@ constexpr long long kMinWork = 1024;        // least work of a CTA, in keys
 // between two others is empty (the join walks the parts of an item one by one).
 static_assert(kMinWork > kOver + (2 * kSnap + 1) * 128, "cuts could meet");
 constexpr float kGrow = 8.f;                // log2 growth of the maximum that forces a rescale
+constexpr int kPoly = 2;                    // of 8 pairs of weights, these go to the FMA pipe
 constexpr float kLog2eF = 1.4426950408889634f;
 
 struct ChunkArgs {
@@ -239,6 +245,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
       "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
       ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8), DBK_I8(v, 16), DBK_I8(v, 24) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16u(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : DBK_R8(v, 0), DBK_R8(v, 8) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16u(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};"
+      ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -251,10 +269,61 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 values in one 64-bit register: one instruction for both (same rounding as single).
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_make(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(f2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of both halves on the FMA pipe, for a share of the weights (the exponential unit gives 16 a
+// clock and SM, and a tile has 16,384): n = round(x) by adding 1.5 * 2^23, which leaves n in the
+// low bits (with 127 added: the exponent field of 2^n after a shift); 2^(x - n) by the minimax
+// polynomial of degree 4 on [-1/2, 1/2], relative error 2^-18.5, far below the rounding of
+// the weight to 16 bits. x <= -127 gives exactly 0, NaN stays NaN.
+__device__ __forceinline__ f2 f2_ex2(f2 x) {
+  float a, b;
+  f2_split(x, a, b);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));       // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+  x = f2_make(a, b);
+  const float big = 12582912.f + 127.f;
+  const f2 t = f2_add(x, f2_make(big, big));
+  const f2 n = f2_add(t, f2_make(-big, -big));
+  const f2 f = f2_fma(n, f2_make(-1.f, -1.f), x);
+  f2 y = f2_make(0.009570102207362652f, 0.009570102207362652f);
+  y = f2_fma(y, f, f2_make(0.05591785907745361f, 0.05591785907745361f));
+  y = f2_fma(y, f, f2_make(0.240247443318367f, 0.240247443318367f));
+  y = f2_fma(y, f, f2_make(0.6931217908859253f, 0.6931217908859253f));
+  y = f2_fma(y, f, f2_make(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb;
+  f2_split(t, ta, tb);
+  const f2 scale = f2_make(__uint_as_float(__float_as_uint(ta) << 23), __uint_as_float(__float_as_uint(tb) << 23));
+  return f2_mul(y, scale);
+}
+
 struct Shared {
   uint64_t full[kRing], empty[kRing];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2], o_full[2], o_free[2], half_ready;
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2], half_ready;
   uint64_t teardown, drain;
   uint32_t tmem;
   volatile int bail;
@@ -281,7 +350,8 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     mbar_init(&sh.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_free[i], 4);
       sh.cut[i] = make_int4(a.batch, 0, 0, 0);
@@ -348,6 +418,9 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   const uint32_t tmem = sh.tmem;
   Walk walk(a, c0, c1);
   Item it;
+
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
 
   if (warp == 8) {
     // ---------------------------------------------------------- TMA: Q, then K and V tiles
@@ -429,25 +502,27 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       }
       __syncwarp();
     };
-    auto weigh = [&](int slot, int k, bool first) {   // O[slot] (+)= P[slot] V
-      if (lane == 0) {
-        const uint64_t dv = desc_mnmajor(smem_u32(ring + (k % kRing) * kTile));
+    // O[slot] (+)= P[slot] V, each half of the keys as soon as its weights are there.
+    auto weigh = [&](int slot, int k, bool first) -> bool {
+      const uint64_t dv = desc_mnmajor(smem_u32(ring + (k % kRing) * kTile));
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, dv + (uint64_t)(s * (2048 >> 4)),
-                 id_o, (first && s == 0) ? 0u : 1u);
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!mbar_wait(&sh.p_full[slot][hf], np[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; return false; }
+        fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int s = 4 * hf; s < 4 * hf + 4; ++s)
+            mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8,
+                   dv + (uint64_t)(s * (2048 >> 4)), id_o, (first && s == 0) ? 0u : 1u);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ++np[slot];
+      return true;
     };
     auto release = [&](int k) {
       if (lane == 0) mma_commit(&sh.empty[k % kRing]);
       __syncwarp();
-    };
-    auto p_ready = [&](int slot) -> bool {
-      if (!mbar_wait(&sh.p_full[slot], np[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; return false; }
-      ++np[slot];
-      fence_after();
-      return true;
     };
     // Keys past the item's last visible one may hold anything (a freed page's NaN): their V
     // rows become zeros, for 0 * NaN would spoil every row.
@@ -481,8 +556,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               fence_after();
             }
             if (s == 0) { if (!(ok = take(kv))) break; clear_tail(kv, it.b0 + j); }
-            if (!(ok = p_ready(s))) break;
-            weigh(s, kv, j == 0);
+            if (!(ok = weigh(s, kv, j == 0))) break;
             if (j + 1 == nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
             else {
               if (s == 0 && !(ok = take(kk))) break;
@@ -519,8 +593,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           }
           if (!(ok = take(n))) break;
           clear_tail(n, it.b0 + j);
-          if (!(ok = p_ready(s))) break;
-          weigh(s, n, j < 2);
+          if (!(ok = weigh(s, n, j < 2))) break;
           release(n);
           ++n;
           if (j + 2 >= nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
@@ -540,7 +613,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     if (lane == 0) mma_commit(&sh.drain);        // every MMA issued has finished
     __syncwarp();
     mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
-  } else {
+  } else if (warp < 8) {
     // ---------------------------------------------------------- softmax, one thread per row
     const int slot = warp >> 2;
     const int r = tid & 127;
@@ -556,6 +629,8 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const int tok = it.two && slot == 1 ? a.T + rt : rt;        // token within the item
       const int vis = max(it.pos + tok + 1, 0);                    // keys this row sees
       const int step = it.two ? 1 : 2;
+      const bool live = r < a.T * a.G && tok < it.ntok;
+      const bool rows = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
       int mine_n = 0;
       bool ok = true;
@@ -563,6 +638,11 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         if (!mbar_wait(&sh.s_full[slot], ns & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
         ++ns;
         fence_after();
+        if (!rows) {                              // no row of this warp is in the item
+          __syncwarp();
+          if (lane == 0) { mbar_arrive(&sh.p_full[slot][0]); mbar_arrive(&sh.p_full[slot][1]); }
+          continue;
+        }
         uint32_t s[4][32];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(t_s + q * 32, s[q]);
@@ -575,6 +655,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             for (int c = 0; c < 32; ++c)
               if (q * 32 + c >= lim) s[q][c] = 0xff800000u;        // -inf
         }
+        __syncwarp();
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 32; c += 2)
@@ -591,39 +672,49 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         } else if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? top : m;
           const float f = grow ? ex2(m - mn) : 1.f;               // m = -inf: 0
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t o[32];
-            tmem_ld32(t_o + slot * 128 + q * 32, o);
+#pragma unroll 1
+          for (int q = 0; q < 8; ++q) {
+            uint32_t o[16];
+            tmem_ld16u(t_o + slot * 128 + q * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-            tmem_st32(t_o + slot * 128 + q * 32, o);
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+            tmem_st16u(t_o + slot * 128 + q * 16, o);
           }
           l *= f;
           m = mn;
         }
         const float nm = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const f2 cs2 = f2_make(a.cs, a.cs), nm2 = f2_make(nm, nm);
+        f2 sum[2] = {0, 0};
 #pragma unroll
-        for (int hq = 0; hq < 2; ++hq) {
+        for (int hf = 0; hf < 2; ++hf) {
           uint32_t p[32];
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
-            const int q = hq * 2 + (c >> 4), e = (2 * c) & 31;
-            const float p0 = ex2(fmaf(__uint_as_float(s[q][e]), a.cs, nm));
-            const float p1 = ex2(fmaf(__uint_as_float(s[q][e + 1]), a.cs, nm));
-            sum[c & 1] += p0;
-            sum[2 + (c & 1)] += p1;
+            const int q = hf * 2 + (c >> 4), e = (2 * c) & 31;
+            f2 x = f2_fma(f2_make(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), cs2, nm2);
+            if ((c & 7) < kPoly) {
+              x = f2_ex2(x);
+            } else {
+              float x0, x1;
+              f2_split(x, x0, x1);
+              x = f2_make(ex2(x0), ex2(x1));
+            }
+            sum[c & 1] = f2_add(sum[c & 1], x);
+            float p0, p1;
+            f2_split(x, p0, p1);
             p[c] = Mma<T>::pack(p0, p1);
           }
-          tmem_st32(t_s + hq * 32, p);
+          tmem_st32(t_s + hf * 32, p);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[slot][hf]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full[slot]);
+        float l0, l1;
+        f2_split(f2_add(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
       if (!ok) break;
 
@@ -659,40 +750,42 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const int sl = 2 * blockIdx.x + (it.b0 > 0 ? 0 : 1);
       if (!whole && tid == 0)
         a.desc[sl] = make_int4(it.tok, it.ntok, it.h, it.b1 == it.nblk ? 2 : 1);
-      const bool live = r < a.T * a.G && tok < it.ntok;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // nothing seen: zeros; NaN stays
       const int prow = slot * kRows + r;
       T* dst = out + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
       float* pdst = a.part_o + ((size_t)sl * a.slot_rows + prow) * kHd;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t o[32];
-        tmem_ld32(t_o + slot * 128 + q * 32, o);
-        tmem_wait_ld();
-        if (joined) {
-          uint32_t o1[32];
-          tmem_ld32(t_o + 128 + q * 32, o1);
+      if (rows) {
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          uint32_t o[32];
+          tmem_ld32(t_o + slot * 128 + q * 32, o);
           tmem_wait_ld();
+          if (joined) {
+            uint32_t o1[32];
+            tmem_ld32(t_o + 128 + q * 32, o1);
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            o[c] = __float_as_uint(__uint_as_float(o[c]) * f0 + __uint_as_float(o1[c]) * f1);
-        }
-        if (live) {
-          if (whole) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 8) {
-              uint4 v;
-              v.x = Mma<T>::pack(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
-              v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
-              v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
-              v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + q * 32 + c) = v;
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; c += 4)
-              *reinterpret_cast<uint4*>(pdst + q * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            for (int c = 0; c < 32; ++c)
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * f0 + __uint_as_float(o1[c]) * f1);
           }
+          if (live) {
+            if (whole) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+                uint4 v;
+                v.x = Mma<T>::pack(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
+                v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+                v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
+                v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
+                *reinterpret_cast<uint4*>(dst + q * 32 + c) = v;
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                *reinterpret_cast<uint4*>(pdst + q * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            }
+          }
+          __syncwarp();
         }
       }
       __syncwarp();
