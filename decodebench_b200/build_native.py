@@ -1,7 +1,7 @@
 """Build the sm_100a kernel library ``decodebench_b200/_lib/libdbk.so`` in-tree.
 
 Each ``csrc/*.cu`` is compiled separately (in parallel) with relocatable device
-code, then device-linked into one shared library exporting the C ABI declared in
+code (but for ``WHOLE_PROGRAM``), then device-linked into one shared library exporting the C ABI declared in
 ``include/dbk.h``. Run ``python -m decodebench_b200.build_native`` or call
 :func:`build`; nvcc cross-compiles, so no GPU is needed.
 """
@@ -31,8 +31,13 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found; the decodebench_b200 kernels need CUDA 12.8+")
 
 
-def _flags(verbose: bool) -> list[str]:
-    f = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC",
+# Built without relocatable device code, for which ptxas ignores setmaxnreg.
+WHOLE_PROGRAM = {"chunk_attn.cu"}
+
+
+def _flags(src: Path, verbose: bool) -> list[str]:
+    rdc = ["-DDBK_WHOLE_PROGRAM"] if src.name in WHOLE_PROGRAM else ["-rdc=true"]
+    f = ARCH + ["-O3", "-lineinfo", "-std=c++17", *rdc, "-Xcompiler", "-fPIC",
                 "--expt-relaxed-constexpr", f"-I{ROOT / 'include'}", f"-I{CSRC}"]
     if verbose:
         f += ["-Xptxas", "-v"]
@@ -46,7 +51,7 @@ def _sources() -> list[Path]:
 def _stale(obj: Path, src: Path) -> bool:
     if not obj.exists():
         return True
-    deps = [src, *CSRC.glob("*.cuh"), *CSRC.glob("*.h"), ROOT / "include" / "dbk.h"]
+    deps = [src, Path(__file__), *CSRC.glob("*.cuh"), *CSRC.glob("*.h"), ROOT / "include" / "dbk.h"]
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 
@@ -61,7 +66,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
         src, obj = pair
         if not force and not _stale(obj, src):
             return ""
-        cmd = [cc, *_flags(verbose), "-c", str(src), "-o", str(obj)]
+        cmd = [cc, *_flags(src, verbose), "-c", str(src), "-o", str(obj)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src.name}:\n{r.stdout}\n{r.stderr}")

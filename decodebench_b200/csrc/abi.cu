@@ -225,12 +225,15 @@ extern "C" int dbk_take_device_error(void) {
   if (e != cudaSuccess) return (int)e;
   e = cudaMemcpyToSymbol(dbk::dbk_device_error, &zero, sizeof(int));
   if (e != cudaSuccess) return (int)e;
-  return v;
+  int w = 0;
+  if (int rc = dbk::chunk_take_error(&w)) return rc;
+  return v ? v : w;
 }
 
 extern "C" int dbk_set_spin_limit(uint32_t polls) {
   const uint32_t v = polls == 0 ? dbk::kSpinLimit : polls;
-  return (int)cudaMemcpyToSymbol(dbk::dbk_spin_limit, &v, sizeof(v));
+  if (int rc = (int)cudaMemcpyToSymbol(dbk::dbk_spin_limit, &v, sizeof(v))) return rc;
+  return dbk::chunk_set_spin_limit(v);
 }
 
 // ---------------------------------------------------------------------------

@@ -34,11 +34,11 @@ constexpr int kHd = 128;                    // head dim
 constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
 constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
 constexpr int kRing = 5;                    // K/V tiles in flight
-constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA warp, MMA warp, 2 idle
-// Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup gives
-// up all but 40, which lets a softmax thread hold its row of S (128 values) without spilling:
-// 256 x 232 + 128 x 40 = 384 x 168.
-constexpr int kRegsSoftmax = 232, kRegsOther = 40;
+constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, tail warps, 1 idle
+// Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup keeps
+// 88 (fewer and its roles spill), which lets a softmax thread hold its row of S (128 values):
+// 256 x 208 + 128 x 88 = 384 x 168.
+constexpr int kRegsSoftmax = 208, kRegsOther = 88;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
@@ -48,7 +48,6 @@ constexpr long long kMinWork = 1024;        // least work of a CTA, in keys
 // between two others is empty (the join walks the parts of an item one by one).
 static_assert(kMinWork > kOver + (2 * kSnap + 1) * 128, "cuts could meet");
 constexpr float kGrow = 8.f;                // log2 growth of the maximum that forces a rescale
-constexpr int kPoly = 2;                    // of 8 pairs of weights, these go to the FMA pipe
 constexpr float kLog2eF = 1.4426950408889634f;
 
 struct ChunkArgs {
@@ -175,34 +174,35 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------ tcgen05 / TMA
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {   // 128-byte swizzle, 8-row groups 1024 B apart
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
+// Shared-memory matrix descriptors, 128-byte swizzle, as a low word (address and leading offset, in
+// units of 16 bytes) over one high word (8-row groups 1024 bytes apart, version, swizzle).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t saddr) { return ((saddr >> 4) & 0x3FFF) | (1u << 16); }
 // MN-major operand (V: 64 head dims per 128-byte row, one row per key): the second 64 dims lie
 // kHalf bytes on (leading offset), the next 8 keys 1024 bytes on (stride offset).
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(kHalf >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t saddr) {
+  return ((saddr >> 4) & 0x3FFF) | ((uint32_t)(kHalf >> 4) << 16);
 }
 __device__ __forceinline__ uint32_t idesc_128x128(bool bf16, bool b_mn) {
   const uint32_t f = bf16 ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((128u >> 3) << 17) |
          ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc,
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                        uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc,
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint32_t b_lo, uint32_t idesc,
                                        uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(ta), "l"(db), "r"(idesc), "r"(acc) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+      ::"r"(d), "r"(ta), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
@@ -289,40 +289,9 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x of both halves on the FMA pipe, for a share of the weights (the exponential unit gives 16 a
-// clock and SM, and a tile has 16,384): n = round(x) by adding 1.5 * 2^23, which leaves n in the
-// low bits (with 127 added: the exponent field of 2^n after a shift); 2^(x - n) by the minimax
-// polynomial of degree 4 on [-1/2, 1/2], relative error 2^-18.5, far below the rounding of
-// the weight to 16 bits. x <= -127 gives exactly 0, NaN stays NaN.
-__device__ __forceinline__ f2 f2_ex2(f2 x) {
-  float a, b;
-  f2_split(x, a, b);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));       // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
-  x = f2_make(a, b);
-  const float big = 12582912.f + 127.f;
-  const f2 t = f2_add(x, f2_make(big, big));
-  const f2 n = f2_add(t, f2_make(-big, -big));
-  const f2 f = f2_fma(n, f2_make(-1.f, -1.f), x);
-  f2 y = f2_make(0.009570102207362652f, 0.009570102207362652f);
-  y = f2_fma(y, f, f2_make(0.05591785907745361f, 0.05591785907745361f));
-  y = f2_fma(y, f, f2_make(0.240247443318367f, 0.240247443318367f));
-  y = f2_fma(y, f, f2_make(0.6931217908859253f, 0.6931217908859253f));
-  y = f2_fma(y, f, f2_make(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb;
-  f2_split(t, ta, tb);
-  const f2 scale = f2_make(__uint_as_float(__float_as_uint(ta) << 23), __uint_as_float(__float_as_uint(tb) << 23));
-  return f2_mul(y, scale);
-}
-
 struct Shared {
   uint64_t full[kRing], empty[kRing];
-  uint64_t q_full, q_empty;
+  uint64_t q_full, q_empty, tail_go, tail;
   uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2], half_ready;
   uint64_t teardown, drain;
   uint32_t tmem;
@@ -348,6 +317,8 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     for (int i = 0; i < kRing; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.tail_go, 1);
+    mbar_init(&sh.tail, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i][0], 4);
@@ -419,9 +390,8 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   Walk walk(a, c0, c1);
   Item it;
 
-  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
   if (warp == 8) {
     // ---------------------------------------------------------- TMA: Q, then K and V tiles
     int n = 0, items = 0;                       // ring tiles issued, items
@@ -479,141 +449,149 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       mbar_wait(&sh.full[k % kRing], (k / kRing) & 1, kDevTimeoutDrain);
     if (items > 0) mbar_wait(&sh.q_full, (items - 1) & 1, kDevTimeoutDrain);
   } else if (warp == 9) {
-    // ---------------------------------------------------------- MMA issue
-    const bool bf = std::is_same<T, __nv_bfloat16>::value;
-    const uint32_t id_s = idesc_128x128(bf, false), id_o = idesc_128x128(bf, true);
-    int n = 0, items = 0;                       // ring tiles taken, items
-    int np[2] = {0, 0}, no[2] = {0, 0};         // P tiles and finished accumulators of each slot
-    auto take = [&](int k) -> bool {            // the k-th ring tile is here
-      if (!mbar_wait(&sh.full[k % kRing], (k / kRing) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
-      fence_after();
-      return true;
-    };
-    auto score = [&](int slot, int k, int qt) { // S[slot] = Q[qt] K^T
-      if (lane == 0) {
-        const uint64_t dq = desc_kmajor(smem_u32(sq + qt * kTile));
-        const uint64_t dk = desc_kmajor(smem_u32(ring + (k % kRing) * kTile));
+    // ---------------------------------------------------------- MMA issue (one thread)
+    if (lane == 0) {
+      const bool bf = std::is_same<T, __nv_bfloat16>::value;
+      const uint32_t id_s = idesc_128x128(bf, false), id_o = idesc_128x128(bf, true);
+      const uint32_t dq = desc_kmajor(smem_u32(sq));
+      const uint32_t dk = desc_kmajor(smem_u32(ring)), dv = desc_mnmajor(smem_u32(ring));
+      int st = 0, ph = 0;                       // ring position
+      int items = 0, tails = 0, np0 = 0, np1 = 0, no0 = 0, no1 = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity, int code) {
+        if (ok && !mbar_wait(bar, parity & 1, code)) { sh.bail = 1; ok = false; }
+        fence_after();
+      };
+      auto advance = [&]() { if (++st == kRing) { st = 0; ph ^= 1; } };
+      auto score = [&](int slot, int stage, int qt) {            // S[slot] = Q[qt] K^T
+        const uint32_t a0 = dq + qt * (kTile >> 4), b0 = dk + stage * (kTile >> 4);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-          const uint64_t o = (uint64_t)((s >> 2) * (kHalf >> 4) + (s & 3) * 2);
-          mma_ss(tmem + slot * 128, dq + o, dk + o, id_s, s != 0);
+          const uint32_t o = (s >> 2) * (kHalf >> 4) + (s & 3) * 2;
+          mma_ss(tmem + slot * 128, a0 + o, b0 + o, id_s, s != 0);
         }
         mma_commit(&sh.s_full[slot]);
-      }
-      __syncwarp();
-    };
-    // O[slot] (+)= P[slot] V, each half of the keys as soon as its weights are there.
-    auto weigh = [&](int slot, int k, bool first) -> bool {
-      const uint64_t dv = desc_mnmajor(smem_u32(ring + (k % kRing) * kTile));
+      };
+      // O[slot] (+)= P[slot] V, each half of the keys as soon as its weights are there.
+      auto weigh = [&](int slot, int stage, bool first, int& np) {
+        const uint32_t b0 = dv + stage * (kTile >> 4);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        if (!mbar_wait(&sh.p_full[slot][hf], np[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; return false; }
-        fence_after();
-        if (lane == 0) {
+        for (int hf = 0; hf < 2; ++hf) {
+          wait(&sh.p_full[slot][hf], np, kDevTimeoutMma);
+          if (ok) {
 #pragma unroll
-          for (int s = 4 * hf; s < 4 * hf + 4; ++s)
-            mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8,
-                   dv + (uint64_t)(s * (2048 >> 4)), id_o, (first && s == 0) ? 0u : 1u);
+            for (int s = 4 * hf; s < 4 * hf + 4; ++s)
+              mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, b0 + s * (2048 >> 4), id_o,
+                     (first && s == 0) ? 0u : 1u);
+          }
         }
-        __syncwarp();
+        ++np;
+      };
+      auto value_tile = [&](int stage, int phase, bool last) {   // V is here, its tail cleared
+        wait(&sh.full[stage], phase, kDevTimeoutFull);
+        if (last && it.kend < it.b1 * kKeys) {
+          mbar_arrive(&sh.tail_go);
+          wait(&sh.tail, tails++, kDevTimeoutFull);
+        }
+      };
+      while (ok && !sh.bail && walk.next(a, it)) {
+        wait(&sh.q_full, items++, kDevTimeoutFull);
+        const int nb = it.b1 - it.b0;
+        wait(&sh.full[st], ph, kDevTimeoutFull);
+        if (!ok) break;
+        score(0, st, 0);
+        if (it.two) {
+          // Ring order: K0 | V0 K1 | V1 K2 | ...; every tile serves both slots.
+          score(1, st, 1);
+          mma_commit(&sh.empty[st]);
+          if (nb == 1) mma_commit(&sh.q_empty);
+          advance();
+          for (int j = 0; ok && j < nb; ++j) {
+            const int vs = st, vp = ph;
+            const bool last = j + 1 == nb;
+            advance();
+            const int ks = st, kp = ph;
+            if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
+            value_tile(vs, vp, last);
+            weigh(0, vs, j == 0, np0);
+            if (last) mma_commit(&sh.o_full[0]);
+            else {
+              wait(&sh.full[ks], kp, kDevTimeoutFull);
+              if (ok) score(0, ks, 0);
+            }
+            if (j == 0 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
+            weigh(1, vs, j == 0, np1);
+            mma_commit(&sh.empty[vs]);
+            if (last) mma_commit(&sh.o_full[1]);
+            else if (ok) {
+              score(1, ks, 1);
+              mma_commit(&sh.empty[ks]);
+              advance();
+              if (j + 2 == nb) mma_commit(&sh.q_empty);
+            }
+          }
+          ++no0;
+          ++no1;
+        } else {
+          // Ring order: K0 K1 | V0 K2 | V1 K3 | ...; block j belongs to slot j & 1.
+          mma_commit(&sh.empty[st]);
+          advance();
+          if (nb > 1) {
+            wait(&sh.full[st], ph, kDevTimeoutFull);
+            if (!ok) break;
+            score(1, st, 0);
+            mma_commit(&sh.empty[st]);
+            advance();
+          }
+          if (nb <= 2) mma_commit(&sh.q_empty);
+          for (int j = 0; ok && j < nb; ++j) {
+            const bool odd = j & 1;
+            if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
+            if (j == 1 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
+            value_tile(st, ph, j + 1 == nb);
+            if (odd) weigh(1, st, j < 2, np1);
+            else weigh(0, st, j < 2, np0);
+            mma_commit(&sh.empty[st]);
+            advance();
+            if (j + 2 >= nb) mma_commit(&sh.o_full[odd]);
+            else {
+              wait(&sh.full[st], ph, kDevTimeoutFull);
+              if (!ok) break;
+              score(odd, st, 0);
+              mma_commit(&sh.empty[st]);
+              advance();
+              if (j + 3 == nb) mma_commit(&sh.q_empty);
+            }
+          }
+          ++no0;
+          if (nb > 1) ++no1;
+        }
       }
-      ++np[slot];
-      return true;
-    };
-    auto release = [&](int k) {
-      if (lane == 0) mma_commit(&sh.empty[k % kRing]);
-      __syncwarp();
-    };
-    // Keys past the item's last visible one may hold anything (a freed page's NaN): their V
-    // rows become zeros, for 0 * NaN would spoil every row.
-    auto clear_tail = [&](int k, int blk) {
-      const int from = it.kend - blk * kKeys;
-      if (from >= kKeys) return;
+      mma_commit(&sh.drain);                    // every MMA issued has finished
+      mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
+    }
+  } else if (warp == 10) {
+    // ---------------------------------------------------------- keys past the last visible one
+    // They may hold anything (a freed page's NaN): their V rows become zeros, for 0 * NaN would
+    // spoil every row. The tile is the item's last in the ring; the MMA thread says when it is here.
+    int n = 0, tails = 0;
+    while (!sh.bail && walk.next(a, it)) {
+      n += 2 * (it.b1 - it.b0);
+      if (it.kend >= it.b1 * kKeys) continue;
+      const int k = n - 1;
+      if (!mbar_wait(&sh.tail_go, tails++ & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
       uint8_t* t = ring + (k % kRing) * kTile;
-      for (int o = max(from, 0) * 128 + lane * 16; o < kHalf; o += 512) {
+      for (int o = max(it.kend - (it.b1 - 1) * kKeys, 0) * 128 + lane * 16; o < kHalf; o += 512) {
         *reinterpret_cast<uint4*>(t + o) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(t + kHalf + o) = make_uint4(0, 0, 0, 0);
       }
       fence_proxy_async_smem();
       __syncwarp();
-    };
-    while (!sh.bail && walk.next(a, it)) {
-      if (!mbar_wait(&sh.q_full, items & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
-      ++items;
-      const int nb = it.b1 - it.b0;
-      bool ok = true;
-      if (it.two) {
-        if (!take(n)) break;
-        score(0, n, 0);
-        score(1, n, 1);
-        release(n);
-        ++n;
-        for (int j = 0; j < nb && ok; ++j) {
-          const int kv = n, kk = n + 1;
-          for (int s = 0; s < 2 && ok; ++s) {
-            if (j == 0 && no[s] > 0) {
-              if (!mbar_wait(&sh.o_free[s], (no[s] - 1) & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
-              fence_after();
-            }
-            if (s == 0) { if (!(ok = take(kv))) break; clear_tail(kv, it.b0 + j); }
-            if (!(ok = weigh(s, kv, j == 0))) break;
-            if (j + 1 == nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
-            else {
-              if (s == 0 && !(ok = take(kk))) break;
-              score(s, kk, s);
-            }
-          }
-          if (!ok) break;
-          release(kv);
-          ++n;
-          if (j + 1 < nb) { release(kk); ++n; }
-          if (j + 2 == nb || nb == 1) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
-        }
-        if (!ok) break;
-        ++no[0];
-        ++no[1];
-      } else {
-        // Ring order: K0 K1 | V0 K2 | V1 K3 | ...; block j belongs to slot j & 1.
-        if (!take(n)) break;
-        score(0, n, 0);
-        release(n);
-        ++n;
-        if (nb > 1) {
-          if (!take(n)) break;
-          score(1, n, 0);
-          release(n);
-          ++n;
-        }
-        if (nb <= 2) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
-        for (int j = 0; j < nb && ok; ++j) {
-          const int s = j & 1;
-          if (j < 2 && no[s] > 0) {
-            if (!mbar_wait(&sh.o_free[s], (no[s] - 1) & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
-            fence_after();
-          }
-          if (!(ok = take(n))) break;
-          clear_tail(n, it.b0 + j);
-          if (!(ok = weigh(s, n, j < 2))) break;
-          release(n);
-          ++n;
-          if (j + 2 >= nb) { if (lane == 0) mma_commit(&sh.o_full[s]); __syncwarp(); }
-          else {
-            if (!(ok = take(n))) break;
-            score(s, n, 0);
-            release(n);
-            ++n;
-            if (j + 3 == nb) { if (lane == 0) mma_commit(&sh.q_empty); __syncwarp(); }
-          }
-        }
-        if (!ok) break;
-        ++no[0];
-        if (nb > 1) ++no[1];
-      }
+      if (lane == 0) mbar_arrive(&sh.tail);
     }
-    if (lane == 0) mma_commit(&sh.drain);        // every MMA issued has finished
-    __syncwarp();
-    mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------------------------------------------------- softmax, one thread per row
     const int slot = warp >> 2;
     const int r = tid & 127;
@@ -656,62 +634,69 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               if (q * 32 + c >= lim) s[q][c] = 0xff800000u;        // -inf
         }
         __syncwarp();
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 32; c += 2)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(s[q][c])), __uint_as_float(s[q][c + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.cs;
-        // The running maximum only follows when it grew by more than kGrow (in log2 units): the
-        // weights then stay below 2^kGrow, exact in fp32 sums and in range for 16 bits, and
-        // most blocks need no pass over O.
-        const bool grow = top > m + kGrow;
-        if (mine_n == 0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? top : m;
-          const float f = grow ? ex2(m - mn) : 1.f;               // m = -inf: 0
-#pragma unroll 1
-          for (int q = 0; q < 8; ++q) {
-            uint32_t o[16];
-            tmem_ld16u(t_o + slot * 128 + q * 16, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-            tmem_st16u(t_o + slot * 128 + q * 16, o);
-          }
-          l *= f;
-          m = mn;
-        }
-        const float nm = m == -INFINITY ? 0.f : -m;
-        const f2 cs2 = f2_make(a.cs, a.cs), nm2 = f2_make(nm, nm);
-        f2 sum[2] = {0, 0};
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t p[32];
+        // The weights of the first 64 keys are formed with the maximum of the blocks before while
+        // the row's maximum is still being found (the exponential unit is what they wait for). Only
+        // if a row's maximum grew by more than kGrow (in log2 units) are they formed again and
+        // O is rescaled: weights stay below 2^kGrow, in range for 16 bits, and a lagging
+        // reference costs a floating-point weight no precision.
+        auto weights = [&](int hf, float nm, uint32_t (&p)[32], f2 (&sum)[2]) {
+          const f2 cs2 = f2_make(a.cs, a.cs), nm2 = f2_make(nm, nm);
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             const int q = hf * 2 + (c >> 4), e = (2 * c) & 31;
-            f2 x = f2_fma(f2_make(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), cs2, nm2);
-            if ((c & 7) < kPoly) {
-              x = f2_ex2(x);
-            } else {
-              float x0, x1;
-              f2_split(x, x0, x1);
-              x = f2_make(ex2(x0), ex2(x1));
-            }
-            sum[c & 1] = f2_add(sum[c & 1], x);
-            float p0, p1;
-            f2_split(x, p0, p1);
-            p[c] = Mma<T>::pack(p0, p1);
+            const f2 x = f2_fma(f2_make(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), cs2, nm2);
+            float x0, x1;
+            f2_split(x, x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            sum[c & 1] = f2_add(sum[c & 1], f2_make(x0, x1));
+            p[c] = Mma<T>::pack(x0, x1);
           }
+        };
+        auto row_max = [&]() {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 32; c += 2)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(s[q][c])), __uint_as_float(s[q][c + 1]));
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.cs;
+        };
+        auto publish = [&](int hf, const uint32_t (&p)[32]) {
           tmem_st32(t_s + hf * 32, p);
           tmem_wait_st();
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot][hf]);
+        };
+        if (mine_n == 0) m = row_max();
+        uint32_t p[32];
+        f2 sum[2] = {0, 0};
+        weights(0, m == -INFINITY ? 0.f : -m, p, sum);
+        const float top = row_max();
+        const bool grow = top > m + kGrow;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? top : m;
+          const float f = grow ? ex2(m - mn) : 1.f;               // m = -inf: 0
+          if (mine_n > 0) {
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+              uint32_t o[16];
+              tmem_ld16u(t_o + slot * 128 + q * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+              tmem_st16u(t_o + slot * 128 + q * 16, o);
+            }
+          }
+          l *= f;
+          m = mn;
+          sum[0] = sum[1] = 0;
+          weights(0, m == -INFINITY ? 0.f : -m, p, sum);
         }
+        publish(0, p);
+        weights(1, m == -INFINITY ? 0.f : -m, p, sum);
+        publish(1, p);
         float l0, l1;
         f2_split(f2_add(sum[0], sum[1]), l0, l1);
         l += l0 + l1;
@@ -885,6 +870,16 @@ int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
 }
 
 }  // namespace
+
+int chunk_take_error(int* code) {
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(code, dbk_device_error, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(dbk_device_error, &zero, sizeof(int));
+  return (int)e;
+}
+int chunk_set_spin_limit(uint32_t polls) {
+  return (int)cudaMemcpyToSymbol(dbk_spin_limit, &polls, sizeof(polls));
+}
 
 }  // namespace dbk
 

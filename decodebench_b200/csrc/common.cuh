@@ -29,7 +29,13 @@ enum DeviceError : int {
   kDevTimeoutGrid = 7,      // waited too long at a grid-wide barrier of a persistent kernel
 };
 
+// A file built as a whole program (DBK_WHOLE_PROGRAM: without relocatable device code, so that
+// setmaxnreg takes effect) has its own flag and budget, which the host side reads and sets too.
+#ifdef DBK_WHOLE_PROGRAM
+static __device__ int dbk_device_error = 0;
+#else
 extern __device__ int dbk_device_error;
+#endif
 
 // Default poll budget for every spin-wait: mbarrier.try_wait suspends for a
 // hardware-chosen interval per poll, so 1<<24 polls is seconds, far beyond
@@ -38,7 +44,11 @@ extern __device__ int dbk_device_error;
 constexpr uint32_t kSpinLimit = 1u << 24;
 // Constant memory: read through the constant cache, so a wait loop pays no
 // global-memory latency for it.
+#ifdef DBK_WHOLE_PROGRAM
+static __constant__ uint32_t dbk_spin_limit = kSpinLimit;
+#else
 extern __constant__ uint32_t dbk_spin_limit;
+#endif
 
 __device__ __forceinline__ uint32_t spin_limit() { return dbk_spin_limit; }
 

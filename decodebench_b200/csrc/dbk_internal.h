@@ -26,6 +26,11 @@ int current_device_info(DeviceInfo* out);
 // device; later calls only check `smem` against the limit).
 int allow_dynamic_smem(const void* kern, const DeviceInfo& dev, size_t smem);
 
+// chunk_attn.cu's own device error flag (read and cleared; the caller has synchronised) and poll
+// budget: that file is built as a whole program (common.cuh).
+int chunk_take_error(int* code);
+int chunk_set_spin_limit(uint32_t polls);
+
 struct PeerSet;   // comm.cuh
 // The peers of an open communicator, for kernels that fuse the all-gather
 // (DBK_EDEVICE unless the current device is the communicator's).
