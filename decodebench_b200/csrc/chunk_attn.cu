@@ -188,25 +188,47 @@ __device__ __forceinline__ uint32_t idesc_128x128(bool bf16, bool b_mn) {
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((128u >> 3) << 17) |
          ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
-                                       uint32_t acc) {
+// The MMA warp runs as a whole, converged, and each of these is issued by the thread that
+// elect.sync chose (`one`). Issued from a branch for one thread instead, with a branch after
+// every wait, 128 x 128 x 16 MMAs went out every 94 cycles in a loop with four waits for 16 of
+// them; this way every 66 (the tensor core takes 64).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint32_t a_lo, uint32_t b_lo,
+                                       uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
       "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi), "r"(one) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint32_t b_lo, uint32_t idesc,
-                                       uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t ta, uint32_t b_lo,
+                                       uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
       "mov.b64 y, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
-      ::"r"(d), "r"(ta), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi) : "memory");
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+      ::"r"(d), "r"(ta), "r"(b_lo), "r"(idesc), "r"(acc), "n"(kDescHi), "r"(one) : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(one) : "memory");
+}
+// Bounded wait without a branch on its outcome: true if the phase completed within `polls`.
+__device__ __forceinline__ bool poll_wait(uint64_t* bar, uint32_t parity, uint32_t polls) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 i;\n\tmov.u32 i, %3;\n\t"
+      "DBK_POLL:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DBK_DONE;\n\t"
+      "sub.u32 i, i, 1;\n\tsetp.ne.u32 q, i, 0;\n\t@q bra DBK_POLL;\n\t"
+      "DBK_DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(polls) : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -449,28 +471,33 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       mbar_wait(&sh.full[k % kRing], (k / kRing) & 1, kDevTimeoutDrain);
     if (items > 0) mbar_wait(&sh.q_full, (items - 1) & 1, kDevTimeoutDrain);
   } else if (warp == 9) {
-    // ---------------------------------------------------------- MMA issue (one thread)
-    if (lane == 0) {
+    // ---------------------------------------------------------- MMA issue
+    {
       const bool bf = std::is_same<T, __nv_bfloat16>::value;
       const uint32_t id_s = idesc_128x128(bf, false), id_o = idesc_128x128(bf, true);
       const uint32_t dq = desc_kmajor(smem_u32(sq));
       const uint32_t dk = desc_kmajor(smem_u32(ring)), dv = desc_mnmajor(smem_u32(ring));
       int st = 0, ph = 0;                       // ring position
       int items = 0, tails = 0, np0 = 0, np1 = 0, no0 = 0, no1 = 0;
-      bool ok = true;
+      const uint32_t one = elect_one();
+      uint32_t polls = spin_limit();            // 1 once a wait has given up
+      int gave_up = 0;
       auto wait = [&](uint64_t* bar, int parity, int code) {
-        if (ok && !mbar_wait(bar, parity & 1, code)) { sh.bail = 1; ok = false; }
+        const bool ok = poll_wait(bar, parity & 1, polls);
+        gave_up = ok || gave_up ? gave_up : code;
+        polls = ok ? polls : 1;
         fence_after();
       };
+      auto failed = [&]() { return __any_sync(0xffffffffu, gave_up != 0); };   // alike in all lanes
       auto advance = [&]() { if (++st == kRing) { st = 0; ph ^= 1; } };
       auto score = [&](int slot, int stage, int qt) {            // S[slot] = Q[qt] K^T
         const uint32_t a0 = dq + qt * (kTile >> 4), b0 = dk + stage * (kTile >> 4);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           const uint32_t o = (s >> 2) * (kHalf >> 4) + (s & 3) * 2;
-          mma_ss(tmem + slot * 128, a0 + o, b0 + o, id_s, s != 0);
+          mma_ss(one, tmem + slot * 128, a0 + o, b0 + o, id_s, s != 0);
         }
-        mma_commit(&sh.s_full[slot]);
+        mma_commit(one, &sh.s_full[slot]);
       };
       // O[slot] (+)= P[slot] V, each half of the keys as soon as its weights are there.
       auto weigh = [&](int slot, int stage, bool first, int& np) {
@@ -478,35 +505,33 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           wait(&sh.p_full[slot][hf], np, kDevTimeoutMma);
-          if (ok) {
 #pragma unroll
-            for (int s = 4 * hf; s < 4 * hf + 4; ++s)
-              mma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, b0 + s * (2048 >> 4), id_o,
-                     (first && s == 0) ? 0u : 1u);
-          }
+          for (int s = 4 * hf; s < 4 * hf + 4; ++s)
+            mma_ts(one, tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, b0 + s * (2048 >> 4), id_o,
+                   (first && s == 0) ? 0u : 1u);
         }
         ++np;
       };
       auto value_tile = [&](int stage, int phase, bool last) {   // V is here, its tail cleared
         wait(&sh.full[stage], phase, kDevTimeoutFull);
         if (last && it.kend < it.b1 * kKeys) {
-          mbar_arrive(&sh.tail_go);
+          if (one) mbar_arrive(&sh.tail_go);
+          __syncwarp();
           wait(&sh.tail, tails++, kDevTimeoutFull);
         }
       };
-      while (ok && !sh.bail && walk.next(a, it)) {
+      while (!failed() && !sh.bail && walk.next(a, it)) {
         wait(&sh.q_full, items++, kDevTimeoutFull);
         const int nb = it.b1 - it.b0;
         wait(&sh.full[st], ph, kDevTimeoutFull);
-        if (!ok) break;
         score(0, st, 0);
         if (it.two) {
           // Ring order: K0 | V0 K1 | V1 K2 | ...; every tile serves both slots.
           score(1, st, 1);
-          mma_commit(&sh.empty[st]);
-          if (nb == 1) mma_commit(&sh.q_empty);
+          mma_commit(one, &sh.empty[st]);
+          if (nb == 1) mma_commit(one, &sh.q_empty);
           advance();
-          for (int j = 0; ok && j < nb; ++j) {
+          for (int j = 0; j < nb && !failed(); ++j) {
             const int vs = st, vp = ph;
             const bool last = j + 1 == nb;
             advance();
@@ -514,60 +539,63 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
             value_tile(vs, vp, last);
             weigh(0, vs, j == 0, np0);
-            if (last) mma_commit(&sh.o_full[0]);
+            if (last) mma_commit(one, &sh.o_full[0]);
             else {
               wait(&sh.full[ks], kp, kDevTimeoutFull);
-              if (ok) score(0, ks, 0);
+              score(0, ks, 0);
             }
             if (j == 0 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
             weigh(1, vs, j == 0, np1);
-            mma_commit(&sh.empty[vs]);
-            if (last) mma_commit(&sh.o_full[1]);
-            else if (ok) {
+            mma_commit(one, &sh.empty[vs]);
+            if (last) mma_commit(one, &sh.o_full[1]);
+            else {
               score(1, ks, 1);
-              mma_commit(&sh.empty[ks]);
+              mma_commit(one, &sh.empty[ks]);
               advance();
-              if (j + 2 == nb) mma_commit(&sh.q_empty);
+              if (j + 2 == nb) mma_commit(one, &sh.q_empty);
             }
           }
           ++no0;
           ++no1;
         } else {
           // Ring order: K0 K1 | V0 K2 | V1 K3 | ...; block j belongs to slot j & 1.
-          mma_commit(&sh.empty[st]);
+          mma_commit(one, &sh.empty[st]);
           advance();
           if (nb > 1) {
             wait(&sh.full[st], ph, kDevTimeoutFull);
-            if (!ok) break;
             score(1, st, 0);
-            mma_commit(&sh.empty[st]);
+            mma_commit(one, &sh.empty[st]);
             advance();
           }
-          if (nb <= 2) mma_commit(&sh.q_empty);
-          for (int j = 0; ok && j < nb; ++j) {
+          if (nb <= 2) mma_commit(one, &sh.q_empty);
+          for (int j = 0; j < nb && !failed(); ++j) {
             const bool odd = j & 1;
             if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
             if (j == 1 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
             value_tile(st, ph, j + 1 == nb);
             if (odd) weigh(1, st, j < 2, np1);
             else weigh(0, st, j < 2, np0);
-            mma_commit(&sh.empty[st]);
+            mma_commit(one, &sh.empty[st]);
             advance();
-            if (j + 2 >= nb) mma_commit(&sh.o_full[odd]);
+            if (j + 2 >= nb) mma_commit(one, &sh.o_full[odd]);
             else {
               wait(&sh.full[st], ph, kDevTimeoutFull);
-              if (!ok) break;
               score(odd, st, 0);
-              mma_commit(&sh.empty[st]);
+              mma_commit(one, &sh.empty[st]);
               advance();
-              if (j + 3 == nb) mma_commit(&sh.q_empty);
+              if (j + 3 == nb) mma_commit(one, &sh.q_empty);
             }
           }
           ++no0;
           if (nb > 1) ++no1;
         }
       }
-      mma_commit(&sh.drain);                    // every MMA issued has finished
+      if (gave_up) {
+        record_error(gave_up);
+        sh.bail = 1;
+      }
+      __syncwarp();
+      mma_commit(one, &sh.drain);                    // every MMA issued has finished
       mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
     }
   } else if (warp == 10) {
