@@ -279,8 +279,15 @@ __device__ __forceinline__ void tmem_st16u(uint32_t addr, const uint32_t (&v)[16
       "%14,%15,%16};"
       ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8) : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// Waits for this thread's TMEM loads; the values pass through it, so no use can move before it.
+#define DBK_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), \
+                      "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : DBK_RW8(v, 0), DBK_RW8(v, 8), DBK_RW8(v, 16), DBK_RW8(v, 24) :: "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : DBK_RW8(v, 0), DBK_RW8(v, 8) :: "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -652,8 +659,9 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         uint32_t s[4][32];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(t_s + q * 32, s[q]);
-        tmem_wait_ld();
-        const int lim = vis - (it.b0 + j) * kKeys;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_wait_ld(s[q]);
+        const int lim = vis - (it.b0 + j) * kKeys;                 // keys this row sees of the block
         if (lim < kKeys) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -711,7 +719,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             for (int q = 0; q < 8; ++q) {
               uint32_t o[16];
               tmem_ld16u(t_o + slot * 128 + q * 16, o);
-              tmem_wait_ld();
+              tmem_wait_ld(o);
 #pragma unroll
               for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
               tmem_st16u(t_o + slot * 128 + q * 16, o);
@@ -772,11 +780,11 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         for (int q = 0; q < 4; ++q) {
           uint32_t o[32];
           tmem_ld32(t_o + slot * 128 + q * 32, o);
-          tmem_wait_ld();
+          tmem_wait_ld(o);
           if (joined) {
             uint32_t o1[32];
             tmem_ld32(t_o + 128 + q * 32, o1);
-            tmem_wait_ld();
+            tmem_wait_ld(o1);
 #pragma unroll
             for (int c = 0; c < 32; ++c)
               o[c] = __float_as_uint(__uint_as_float(o[c]) * f0 + __uint_as_float(o1[c]) * f1);
