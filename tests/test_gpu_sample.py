@@ -84,6 +84,13 @@ def test_filters(dt, batch, vocab):
     check(x, u, temperature=1.1, top_k=40, top_p=0.8, min_p=0.1)
 
 
+def test_small_min_p():
+    x, u = rows(6, 20000, F32, seed=3, spread=1.5)
+    for mp in (1e-9, 1e-5, 2.0 ** -14, 1.1e-4, 2.0 ** -13, 1e-3):
+        check(x, u, min_p=mp, temperature=1.7)
+        check(x, u, min_p=mp, top_p=0.9)
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_flat_and_long_tails(dt):
     """Flat rows (every weight counts), cuts deep in the tail, sharp temperatures."""
