@@ -36,9 +36,9 @@ constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
 constexpr int kRing = 5;                    // K/V tiles in flight
 constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, tail warps, 1 idle
 // Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup keeps
-// 88 (fewer and its roles spill), which lets a softmax thread hold its row of S (128 values):
-// 256 x 208 + 128 x 88 = 384 x 168.
-constexpr int kRegsSoftmax = 208, kRegsOther = 88;
+// 72 (fewer and its roles spill), which lets a softmax thread hold its row of S (128 values):
+// 256 x 216 + 128 x 72 = 384 x 168.
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
