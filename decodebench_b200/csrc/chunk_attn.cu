@@ -42,6 +42,7 @@ constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
+constexpr int kOneTile = 5;                 // cost of a key of a one-tile item, in eighths
 constexpr int kSnap = 2;                    // a cut this near an item's end moves to the end
 constexpr long long kMinWork = 1024;        // least work of a CTA, in keys
 // Neighbouring cuts are at least kMinWork apart and move by less than half of that, so no part
@@ -56,7 +57,7 @@ struct ChunkArgs {
   const int32_t* lens;       // [batch] tokens in the cache, the new ones included
   const int32_t* pages;      // [batch, max_pages] or nullptr (contiguous)
   void* out;
-  float* part_o;             // [2 * grid][slot_rows][128]
+  float* part_o;             // [2 * grid][32][slot_rows][4]: column fours, rows, columns
   float2* part_ml;           // [2 * grid][slot_rows] (maximum in log2 units, sum)
   int4* desc;                // [2 * grid] {first token, tokens, kv head, 0 | 1 goes on | 2 last}
   int batch, tokens, hq, hkv, G, T;
@@ -88,7 +89,7 @@ __device__ __forceinline__ Seq load_seq(const ChunkArgs& a, int b) {
   if (s.n > 0) {
     const int rem = s.n - (s.items - 1) * 2 * a.T;
     const long long seen = max(s.len, s.n);
-    s.per_head = cost_before(a, s, s.items - 1) + kOver + (rem <= a.T ? (seen + 1) / 2 : seen);
+    s.per_head = cost_before(a, s, s.items - 1) + kOver + (rem <= a.T ? (seen * kOneTile + 7) / 8 : seen);
   }
   return s;
 }
@@ -112,21 +113,25 @@ __device__ __forceinline__ void item_shape(const ChunkArgs& a, const Seq& s, int
   it.nblk = max(1, (it.kend + kKeys - 1) / kKeys);
 }
 
-// First (b, h, item, block) of the part that starts at cost `off` inside sequence b.
-__device__ int4 locate(const ChunkArgs& a, int b, long long off) {
-  Seq s = load_seq(a, b);
-  int h = (int)(off / s.per_head);
+// First (b, h, item, block) of the part that starts at cost `off` inside sequence b, and that
+// sequence. Quotients and the root of the quadratic cost_before come from 64-bit floats and are
+// then put right: an integer division or a search takes thousands of cycles before a CTA's start.
+__device__ __forceinline__ int4 locate(const ChunkArgs& a, int b, long long off, Seq& s) {
+  s = load_seq(a, b);
+  int h = (int)((double)off / (double)s.per_head);
   off -= h * s.per_head;
-  int lo = 0, hi = s.items - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cost_before(a, s, mid) <= off) lo = mid; else hi = mid - 1;
-  }
-  int i = lo;
+  if (off < 0) { --h; off += s.per_head; }
+  else if (off >= s.per_head) { ++h; off -= s.per_head; }
+  const double base = (double)(max(s.len - s.n, 0) + kOver) + a.T, w = (double)a.T;
+  int i = (int)((sqrt(base * base + 4.0 * w * (double)off) - base) / (2.0 * w));
+  i = min(max(i, 0), s.items - 1);
+  while (i > 0 && cost_before(a, s, i) > off) --i;
+  while (i + 1 < s.items && cost_before(a, s, i + 1) <= off) ++i;
   off -= cost_before(a, s, i);
   Item it;
   item_shape(a, s, i, it);
-  int blk = (int)min((off * (it.two ? 1 : 2) + kKeys / 2) / kKeys, (long long)INT_MAX / 2);
+  const int left = (int)min(off, (long long)INT_MAX / 16);
+  int blk = it.two ? (left + kKeys / 2) / kKeys : (left * 8 + kOneTile * kKeys / 2) / (kOneTile * kKeys);
   if (blk < kSnap) blk = 0;
   else if (blk + kSnap > it.nblk) {
     blk = 0;
@@ -134,7 +139,7 @@ __device__ int4 locate(const ChunkArgs& a, int b, long long off) {
       i = 0;
       if (++h == a.hkv) {
         h = 0;
-        do ++b; while (b < a.batch && load_seq(a, b).n == 0);
+        do { if (++b >= a.batch) break; s = load_seq(a, b); } while (s.n == 0);
       }
     }
   }
@@ -145,9 +150,7 @@ __device__ int4 locate(const ChunkArgs& a, int b, long long off) {
 struct Walk {
   int4 at, end;
   Seq s;
-  __device__ __forceinline__ Walk(const ChunkArgs& a, int4 from, int4 to) : at(from), end(to) {
-    if (at.x < a.batch) s = load_seq(a, at.x);
-  }
+  __device__ __forceinline__ Walk(int4 from, int4 to, const Seq& first) : at(from), end(to), s(first) {}
   __device__ __forceinline__ bool next(const ChunkArgs& a, Item& it) {
     if (at.x >= a.batch) return false;
     const bool last = at.x == end.x && at.y == end.y && at.z == end.z;
@@ -292,6 +295,11 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[16]) {
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void st_32(void* p, const uint32_t (&v)[8]) {   // one 32-byte sector
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -328,6 +336,7 @@ struct Shared {
   long long wsum[kThreadsCa / 32], before[kThreadsCa / 32];
   long long total;
   int4 cut[2];
+  Seq first;                 // the sequence of the first cut
   float2 half_ml[kRows];     // the second warpgroup's maximum and sum (one-tile items)
 };
 
@@ -397,18 +406,24 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   }
   __syncthreads();
   const long long W = sh.total;
-  const long long parts = min((long long)gridDim.x, max(1ll, W / kMinWork));
+  const int parts = (int)min((long long)gridDim.x, max(1ll, W / kMinWork));   // (a power of two)
   {
     const long long lo = sh.before[warp] + inc - mine;
+    const double part = (double)W / (double)parts;
 #pragma unroll 1
     for (int e = 0; e < 2; ++e) {
-      const long long c = blockIdx.x + e;
+      const int c = blockIdx.x + e;
       if (c >= parts) break;
-      long long w = W * c / parts - lo;
+      long long w = (long long)(part * c) - lo;
       if (mine == 0 || w < 0 || w >= mine) continue;
       for (int b = sb0; b < sb1; ++b) {
         const long long cost = load_seq(a, b).per_head * a.hkv;
-        if (w < cost) { sh.cut[e] = locate(a, b, w); break; }
+        if (w < cost) {
+          Seq s;
+          sh.cut[e] = locate(a, b, w, s);
+          if (e == 0) sh.first = s;
+          break;
+        }
         w -= cost;
       }
     }
@@ -416,7 +431,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   __syncthreads();
   const int4 c0 = sh.cut[0], c1 = sh.cut[1];
   const uint32_t tmem = sh.tmem;
-  Walk walk(a, c0, c1);
+  Walk walk(c0, c1, sh.first);
   Item it;
 
   if (warp >= 8) {
@@ -427,17 +442,6 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     const int pieces = kKeys / a.box;
     const uint32_t piece_bytes = (uint32_t)a.box * 256;
     while (!sh.bail && walk.next(a, it)) {
-      if (items > 0 && !mbar_wait(&sh.q_empty, (items - 1) & 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
-      if (lane == 0) {
-        const uint32_t qb = (uint32_t)(a.T * a.G) * 256;
-        mbar_arrive_expect_tx(&sh.q_full, it.two ? 2 * qb : qb);
-        for (int t = 0; t < (it.two ? 2 : 1); ++t)
-          for (int hf = 0; hf < 2; ++hf)
-            tma_3d(sq + t * kTile + hf * kHalf, &a.qmap, hf * 64, it.h * a.G, it.tok + t * a.T,
-                   &sh.q_full);
-      }
-      __syncwarp();
-      ++items;
       // Lane p < pieces brings the p-th piece of each block; `row` is its row in the cache.
       auto row_of = [&](int blk) -> int {
         const int tok = blk * kKeys + lane * a.box;
@@ -464,7 +468,18 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       };
       const int ahead = it.two ? 1 : 2;
       int r0 = row_of(it.b0), r1 = row_of(it.b0 + 1), r2 = row_of(it.b0 + 2);
-      if (!issue(&a.kmap, it.b0, r0)) break;
+      if (!issue(&a.kmap, it.b0, r0)) break;      // the ring has room before the last item's Q is free
+      if (items > 0 && !mbar_wait(&sh.q_empty, (items - 1) & 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
+      if (lane == 0) {
+        const uint32_t qb = (uint32_t)(a.T * a.G) * 256;
+        mbar_arrive_expect_tx(&sh.q_full, it.two ? 2 * qb : qb);
+        for (int t = 0; t < (it.two ? 2 : 1); ++t)
+          for (int hf = 0; hf < 2; ++hf)
+            tma_3d(sq + t * kTile + hf * kHalf, &a.qmap, hf * 64, it.h * a.G, it.tok + t * a.T,
+                   &sh.q_full);
+      }
+      __syncwarp();
+      ++items;
       if (ahead == 2 && it.b0 + 1 < it.b1 && !issue(&a.kmap, it.b0 + 1, r1)) break;
       for (int j = it.b0; j < it.b1; ++j) {
         const int r3 = row_of(j + 3);
@@ -774,7 +789,8 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // nothing seen: zeros; NaN stays
       const int prow = slot * kRows + r;
       T* dst = out + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
-      float* pdst = a.part_o + ((size_t)sl * a.slot_rows + prow) * kHd;
+      float* pdst = a.part_o + (size_t)sl * a.slot_rows * kHd + prow * 4;    // [32 column fours][rows][4]
+      const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
       if (rows) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
@@ -792,18 +808,22 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           if (live) {
             if (whole) {
 #pragma unroll
-              for (int c = 0; c < 32; c += 8) {
-                uint4 v;
-                v.x = Mma<T>::pack(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv);
-                v.y = Mma<T>::pack(__uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
-                v.z = Mma<T>::pack(__uint_as_float(o[c + 4]) * inv, __uint_as_float(o[c + 5]) * inv);
-                v.w = Mma<T>::pack(__uint_as_float(o[c + 6]) * inv, __uint_as_float(o[c + 7]) * inv);
-                *reinterpret_cast<uint4*>(dst + q * 32 + c) = v;
+              for (int c = 0; c < 32; c += 16) {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  v[e] = Mma<T>::pack(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+                if (wide) st_32(dst + q * 32 + c, v);
+                else {
+                  *reinterpret_cast<uint4*>(dst + q * 32 + c) = make_uint4(v[0], v[1], v[2], v[3]);
+                  *reinterpret_cast<uint4*>(dst + q * 32 + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                }
               }
             } else {
 #pragma unroll
               for (int c = 0; c < 32; c += 4)
-                *reinterpret_cast<uint4*>(pdst + q * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                *reinterpret_cast<uint4*>(pdst + (size_t)(q * 8 + c / 4) * a.slot_rows * 4) =
+                    make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
             }
           }
           __syncwarp();
@@ -830,18 +850,21 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   }
 }
 
-// Joins the partials of the items that CTA cuts went through. Block (c, y): the item whose
-// first piece CTA c left, rows 8 warps at a time; a row's pieces are weighted by
-// 2^(m - max m) in the order of the keys.
-constexpr int kJoinSlices = 8;
+// Joins the partials of the items that CTA cuts went through. Block (c, y): rows 32 y .. 32 y + 31 of
+// the item whose first piece CTA c left; a row's pieces are weighted by 2^(m - max m) in the
+// order of the keys. A lane has a row and a warp four of its column fours at a time, so that
+// every load is 512 contiguous bytes; the result turns through shared memory into whole rows.
+constexpr int kJoinRows = 32;
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
+  __shared__ float turn[kJoinRows][kHd + 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int4 d = __ldcg(a.desc + 2 * c + 1);
-  if (d.w != 1) return;
+  const int r0 = blockIdx.y * kJoinRows;
+  if (d.w != 1 || r0 >= a.slot_rows || r0 >= (d.y > a.T ? 2 * kRows : kRows)) return;
   int pieces = 1;
   while (c + pieces < (int)gridDim.x) {
     const int f = __ldcg(&a.desc[2 * (c + pieces)].w);
@@ -850,40 +873,50 @@ __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __gri
     if (f == 2) break;
   }
   auto slot_of = [&](int p) { return p == 0 ? 2 * c + 1 : 2 * (c + p); };
-  const int rows = d.y > a.T ? 2 * kRows : kRows;
-  for (int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); r < rows; r += kJoinSlices * kJoinWarps) {
-    const int rr = r & (kRows - 1), rt = rr / a.G;
-    const int tok = (r >> 7) * a.T + rt;
-    if (rr >= a.T * a.G || tok >= d.y) continue;
-    float m = -INFINITY;
-    for (int p = lane; p < pieces; p += 32)
+  auto token_of = [&](int r) {                     // of row r within the item; -1: no such row
+    const int rr = r & (kRows - 1), tok = (r >> 7) * a.T + rr / a.G;
+    return r < a.slot_rows && rr < a.T * a.G && tok < d.y ? tok : -1;
+  };
+  const int r = r0 + lane;
+  const bool live = token_of(r) >= 0;
+  float m = -INFINITY;
+  if (live)
+    for (int p = 0; p < pieces; ++p)
       m = fmaxf(m, __ldcg(a.part_ml + (size_t)slot_of(p) * a.slot_rows + r).x);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < pieces; p0 += 32) {
-      float w = 0.f, lw = 0.f;
-      if (p0 + lane < pieces) {
-        const float2 ml = __ldcg(a.part_ml + (size_t)slot_of(p0 + lane) * a.slot_rows + r);
-        w = ex2(ml.x - ref);
-        lw = ml.y * w;
-      }
-      l += warp_sum(lw);
-      const int cnt = min(32, pieces - p0);
-#pragma unroll 4
-      for (int p = 0; p < cnt; ++p) {
-        const float wp = __shfl_sync(0xffffffffu, w, p);
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(
-            a.part_o + ((size_t)slot_of(p0 + p) * a.slot_rows + r) * kHd) + lane);
-        acc.x += o.x * wp; acc.y += o.y * wp; acc.z += o.z * wp; acc.w += o.w * wp;
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+#pragma unroll 2
+    for (int p = 0; p < pieces; ++p) {
+      const float2 ml = __ldcg(a.part_ml + (size_t)slot_of(p) * a.slot_rows + r);
+      const float w = ex2(ml.x - ref);
+      l += ml.y * w;
+      const float4* src = reinterpret_cast<const float4*>(a.part_o) + (size_t)slot_of(p) * 32 * a.slot_rows + r;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 o = __ldcg(src + (size_t)(warp * 4 + q) * a.slot_rows);
+        acc[q].x += o.x * w; acc[q].y += o.y * w; acc[q].z += o.z * w; acc[q].w += o.w * w;
       }
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    T* dst = static_cast<T*>(a.out) + ((size_t)(d.x + tok) * a.hq + d.z * a.G + (rr - rt * a.G)) * kHd;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<float4*>(&turn[lane][(warp * 4 + q) * 4]) =
+          make_float4(acc[q].x * inv, acc[q].y * inv, acc[q].z * inv, acc[q].w * inv);
+  }
+  __syncthreads();
+  for (int k = warp; k < kJoinRows; k += kJoinWarps) {
+    const int tok = token_of(r0 + k);
+    if (tok < 0) continue;
+    const int rg = ((r0 + k) & (kRows - 1)) % a.G;
+    const float4 o = *reinterpret_cast<const float4*>(&turn[k][lane * 4]);
     uint2 v;
-    v.x = Mma<T>::pack(acc.x * inv, acc.y * inv);
-    v.y = Mma<T>::pack(acc.z * inv, acc.w * inv);
+    v.x = Mma<T>::pack(o.x, o.y);
+    v.y = Mma<T>::pack(o.z, o.w);
+    T* dst = static_cast<T*>(a.out) + ((size_t)(d.x + tok) * a.hq + d.z * a.G + rg) * kHd;
     *reinterpret_cast<uint2*>(dst + lane * 4) = v;
   }
 }
@@ -902,7 +935,8 @@ int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
   if (int rc = allow_dynamic_smem(kern, dev, smem)) return rc;
   if (int rc = launch_pdl(kern, dim3(dev.num_sms), dim3(kThreadsCa), smem, st, &a)) return rc;
   return launch_pdl(reinterpret_cast<const void*>(&chunk_join_kernel<T>),
-                    dim3(dev.num_sms, kJoinSlices), dim3(kJoinWarps * 32), 0, st, &a);
+                    dim3(dev.num_sms, (a.slot_rows + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0,
+                    st, &a);
 }
 
 }  // namespace
