@@ -852,13 +852,14 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
 
 // Joins the partials of the items that CTA cuts went through. Block (c, y): rows 32 y .. 32 y + 31 of
 // the item whose first piece CTA c left; a row's pieces are weighted by 2^(m - max m) in the
-// order of the keys. A lane has a row and a warp four of its column fours at a time, so that
-// every load is 512 contiguous bytes; the result turns through shared memory into whole rows.
+// order of the keys. A lane has a row and a warp NC of its column fours, so that every load is 512
+// contiguous bytes; the result turns through shared memory into whole rows. NC = 1 spreads the
+// columns over four blocks, for few rows whose pieces are many.
 constexpr int kJoinRows = 32;
 constexpr int kJoinWarps = 8;
-template <typename T>
+template <typename T, int NC>
 __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __grid_constant__ ChunkArgs a) {
-  __shared__ float turn[kJoinRows][kHd + 4];
+  __shared__ float turn[kJoinRows][kJoinWarps * NC * 4 + 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -879,45 +880,50 @@ __global__ void __launch_bounds__(kJoinWarps * 32) chunk_join_kernel(const __gri
   };
   const int r = r0 + lane;
   const bool live = token_of(r) >= 0;
+  const float2* ml = a.part_ml + r;
   float m = -INFINITY;
-  if (live)
-    for (int p = 0; p < pieces; ++p)
-      m = fmaxf(m, __ldcg(a.part_ml + (size_t)slot_of(p) * a.slot_rows + r).x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 acc[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
-#pragma unroll 2
+#pragma unroll 8
+    for (int p = 0; p < pieces; ++p) m = fmaxf(m, __ldcg(ml + (size_t)slot_of(p) * a.slot_rows).x);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  constexpr int kCols = kJoinWarps * NC * 4;       // columns of this block
+  const int four0 = (blockIdx.z * kJoinWarps + warp) * NC;
+  float l = 0.f;
+  float4 acc[NC];
+#pragma unroll
+  for (int q = 0; q < NC; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+#pragma unroll (NC == 1 ? 8 : 2)
     for (int p = 0; p < pieces; ++p) {
-      const float2 ml = __ldcg(a.part_ml + (size_t)slot_of(p) * a.slot_rows + r);
-      const float w = ex2(ml.x - ref);
-      l += ml.y * w;
+      const float2 s = __ldcg(ml + (size_t)slot_of(p) * a.slot_rows);
+      const float w = ex2(s.x - ref);
+      l += s.y * w;
       const float4* src = reinterpret_cast<const float4*>(a.part_o) + (size_t)slot_of(p) * 32 * a.slot_rows + r;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 o = __ldcg(src + (size_t)(warp * 4 + q) * a.slot_rows);
+      for (int q = 0; q < NC; ++q) {
+        const float4 o = __ldcg(src + (size_t)(four0 + q) * a.slot_rows);
         acc[q].x += o.x * w; acc[q].y += o.y * w; acc[q].z += o.z * w; acc[q].w += o.w * w;
       }
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<float4*>(&turn[lane][(warp * 4 + q) * 4]) =
+    for (int q = 0; q < NC; ++q)
+      *reinterpret_cast<float4*>(&turn[lane][(warp * NC + q) * 4]) =
           make_float4(acc[q].x * inv, acc[q].y * inv, acc[q].z * inv, acc[q].w * inv);
   }
   __syncthreads();
-  for (int k = warp; k < kJoinRows; k += kJoinWarps) {
-    const int tok = token_of(r0 + k);
+  constexpr int kLanes = kCols / 4;                // lanes of a row's columns
+  for (int k = threadIdx.x / kLanes; k < kJoinRows; k += kJoinWarps * 32 / kLanes) {
+    const int tok = token_of(r0 + k), e = (threadIdx.x % kLanes) * 4;
     if (tok < 0) continue;
     const int rg = ((r0 + k) & (kRows - 1)) % a.G;
-    const float4 o = *reinterpret_cast<const float4*>(&turn[k][lane * 4]);
+    const float4 o = *reinterpret_cast<const float4*>(&turn[k][e]);
     uint2 v;
     v.x = Mma<T>::pack(o.x, o.y);
     v.y = Mma<T>::pack(o.z, o.w);
     T* dst = static_cast<T*>(a.out) + ((size_t)(d.x + tok) * a.hq + d.z * a.G + rg) * kHd;
-    *reinterpret_cast<uint2*>(dst + lane * 4) = v;
+    *reinterpret_cast<uint2*>(dst + blockIdx.z * kCols + e) = v;
   }
 }
 
@@ -934,9 +940,11 @@ int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
   const void* kern = reinterpret_cast<const void*>(&chunk_attention_kernel<T>);
   if (int rc = allow_dynamic_smem(kern, dev, smem)) return rc;
   if (int rc = launch_pdl(kern, dim3(dev.num_sms), dim3(kThreadsCa), smem, st, &a)) return rc;
-  return launch_pdl(reinterpret_cast<const void*>(&chunk_join_kernel<T>),
-                    dim3(dev.num_sms, (a.slot_rows + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0,
-                    st, &a);
+  const unsigned y = (a.slot_rows + kJoinRows - 1) / kJoinRows;
+  const bool few = a.slot_rows <= kRows;
+  return launch_pdl(few ? reinterpret_cast<const void*>(&chunk_join_kernel<T, 1>)
+                        : reinterpret_cast<const void*>(&chunk_join_kernel<T, 4>),
+                    dim3(dev.num_sms, y, few ? 4 : 1), dim3(kJoinWarps * 32), 0, st, &a);
 }
 
 }  // namespace

@@ -11,7 +11,6 @@ missing kernel library, raises.
 
 from __future__ import annotations
 
-import contextlib
 import math
 import os
 import threading
@@ -516,12 +515,29 @@ class PagePlan(NamedTuple):
     used: torch.Tensor          # int32 [1]: free pages the step needs
 
 
-_same_device = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` current for a launch when it is not."""
-    return _same_device if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _launch(fn: str, dev: torch.device, *args) -> None:
+    """Calls ``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current."""
+    call = getattr(N.load(), fn)
+    if _current_device() == dev.index:
+        status = call(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = call(*args, _stream(dev))
+    if status != 0:
+        raise N.DbkError(fn, status)
+
+
+def _cuda_device(*ts: torch.Tensor) -> torch.device:
+    """As :func:`_need_cuda` for tensors that are all given, with one call per check (these calls'
+    kernels take a few microseconds)."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index or not t.is_contiguous():
+            return _need_cuda(*ts)
+    return ts[0].device if index >= 0 else _need_cuda(*ts)
 
 
 def _check_i32(name: str, t: torch.Tensor, numel: int) -> None:
@@ -540,7 +556,7 @@ def page_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.
     ``n_tokens`` is the packed length of the step's tensors; rows behind the last token get
     position 0 and slot -1. Where the list or the table is too short, table entries and slots
     become -1, and ``used`` tells how many pages the step needs. See ``dbk_page_plan``."""
-    dev = _need_cuda(ctx_lens, new_lens, free_pages, page_table)
+    dev = _cuda_device(ctx_lens, new_lens, free_pages, page_table)
     if page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise ValueError("page_table must be int32 [batch, max_pages]")
     batch, max_pages = page_table.shape
@@ -550,16 +566,15 @@ def page_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.
         raise ValueError("free_pages must be int32")
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
-    lens = torch.empty(batch, dtype=torch.int32, device=dev)
-    cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
-    pos = torch.empty(n_tokens, dtype=torch.int32, device=dev)
     slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
-    used = torch.empty(1, dtype=torch.int32, device=dev)
-    with _on(dev):
-        N.check("dbk_page_plan", N.load().dbk_page_plan(
-            ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), page_table.data_ptr(),
-            lens.data_ptr(), cu.data_ptr(), pos.data_ptr(), slots.data_ptr(), used.data_ptr(),
-            batch, free_pages.numel(), int(page_size), max_pages, int(n_tokens), _stream(dev)))
+    pos, lens, cu, used = torch.empty(
+        n_tokens + 2 * batch + 2, dtype=torch.int32, device=dev).split_with_sizes(
+        [n_tokens, batch, batch + 1, 1])
+    at = used.data_ptr() - 4 * (n_tokens + 2 * batch + 1)      # (an empty tensor has no address)
+    _launch("dbk_page_plan", dev, ctx_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(),
+            page_table.data_ptr(), at + 4 * n_tokens, at + 4 * (n_tokens + batch), at,
+            slots.data_ptr(), at + 4 * (n_tokens + 2 * batch + 1), batch, free_pages.numel(),
+            page_size, max_pages, n_tokens)
     return PagePlan(lens, cu, pos, slots, used)
 
 
@@ -574,7 +589,7 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
     cache [batch, Hkv, max_len, 128] has slot b * max_len + position). k and v are written into
     the caches in place, rows with a slot outside the cache (-1) are not; returns q
     [tokens, Hq, 128], rotated. Slots must differ from one another."""
-    dev = _need_cuda(qkv, positions, slots, inv_freq, k_cache, v_cache)
+    dev = _cuda_device(qkv, positions, slots, inv_freq, k_cache, v_cache)
     _check_out(out, dev)
     dt = _dtype_code(qkv)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_kv_heads:
@@ -590,14 +605,15 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
         raise ValueError(f"slots must be int64 with {n} elements")
     if inv_freq.dtype != torch.float32 or inv_freq.numel() != D // 2:
         raise ValueError(f"inv_freq must be float32 [{D // 2}]")
-    q = out if out is not None else torch.empty(n, n_q_heads, D, dtype=qkv.dtype, device=dev)
-    if q.dtype != qkv.dtype or q.numel() != n * n_q_heads * D:
-        raise ValueError(f"out must be [{n}, {n_q_heads}, {D}] of qkv's dtype")
-    with _on(dev):
-        N.check("dbk_rope_append", N.load().dbk_rope_append(
-            qkv.data_ptr(), positions.data_ptr(), slots.data_ptr(), inv_freq.data_ptr(),
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n, n_q_heads, n_kv_heads, D,
-            pages, page_size, dt, _stream(dev)))
+    if out is None:
+        q = torch.empty(n, n_q_heads, D, dtype=qkv.dtype, device=dev)
+    else:
+        q = out
+        if q.dtype != qkv.dtype or q.numel() != n * n_q_heads * D:
+            raise ValueError(f"out must be [{n}, {n_q_heads}, {D}] of qkv's dtype")
+    _launch("dbk_rope_append", dev, qkv.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+            inv_freq.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n,
+            n_q_heads, n_kv_heads, D, pages, page_size, dt)
     return q
 
 
@@ -615,7 +631,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (``page_table`` int32 [batch, max_pages]): k/v [pages, Hkv, page_size, 128], page_size a
     multiple of 8; contiguous: [batch, Hkv, max_len, 128]. ``scale`` (> 0) defaults to
     1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` are left as they were."""
-    dev = _need_cuda(q, k_cache, v_cache, cu_seqlens, seq_lens, page_table)
+    dev = (_cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens) if page_table is None else
+           _cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens, page_table))
     _check_out(out, dev)
     dt = _dtype_code(q)
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
@@ -652,12 +669,10 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
     elif workspace.dtype != torch.uint8 or workspace.device != dev or workspace.numel() < nb:
         raise ValueError(f"workspace must be a uint8 tensor of >= {nb} bytes on {dev}")
-    with _on(dev):
-        N.check("dbk_chunk_attention", lib.dbk_chunk_attention(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cu_seqlens.data_ptr(),
-            seq_lens.data_ptr(), _ptr(page_table), o.data_ptr(), tokens, batch, hq, hkv, D,
-            pages, page_size, max_pages, float(scale), dt, workspace.data_ptr(), nb,
-            _stream(dev)))
+    _launch("dbk_chunk_attention", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            cu_seqlens.data_ptr(), seq_lens.data_ptr(), _ptr(page_table), o.data_ptr(), tokens,
+            batch, hq, hkv, D, pages, page_size, max_pages, float(scale), dt,
+            workspace.data_ptr(), nb)
     return o
 
 
@@ -685,8 +700,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
     [0, 1)) times their sum; temperature <= 0 takes the largest logit. Each parameter is a
     number or a tensor [batch] (fp32, ``top_k`` int32; None, top_k <= 0, top_p >= 1 and
     min_p <= 0 are off). NaN counts as -inf; a row of nothing but -inf gives -1."""
-    dev = _need_cuda(logits, uniforms, *(t for t in (temperature, top_k, top_p, min_p)
-                                         if isinstance(t, torch.Tensor)))
+    dev = _cuda_device(logits, uniforms, *[t for t in (temperature, top_k, top_p, min_p)
+                                           if isinstance(t, torch.Tensor)])
     if logits.dim() != 2:
         raise ValueError("logits must be [batch, vocab]")
     dt = N.DBK_F32 if logits.dtype == torch.float32 else _dtype_code(logits)
@@ -702,11 +717,9 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
     if o.dtype != torch.int64 or o.numel() != batch:
         raise ValueError(f"out must be int64 with {batch} elements")
     _check_out(out, dev)
-    with _on(dev):
-        N.check("dbk_sample", N.load().dbk_sample(
-            logits.data_ptr(), uniforms.data_ptr(), _ptr(t), _ptr(k), _ptr(p), _ptr(m),
-            o.data_ptr(), batch, vocab, float(t_all), max(0, min(int(k_all), 2 ** 31 - 1)),
-            float(p_all), float(m_all), dt, _stream(dev)))
+    _launch("dbk_sample", dev, logits.data_ptr(), uniforms.data_ptr(), _ptr(t), _ptr(k), _ptr(p),
+            _ptr(m), o.data_ptr(), batch, vocab, float(t_all), max(0, min(int(k_all), 2 ** 31 - 1)),
+            float(p_all), float(m_all), dt)
     return o
 
 
