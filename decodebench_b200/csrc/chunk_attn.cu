@@ -34,12 +34,13 @@ constexpr int kHd = 128;                    // head dim
 constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
 constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
 constexpr int kRing = 5;                    // K/V tiles in flight
-constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, tail warps, 1 idle
+constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, tail, item warps
 // Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup keeps
 // 72 (fewer and its roles spill), which lets a softmax thread hold its row of S (128 values):
 // 256 x 216 + 128 x 72 = 384 x 168.
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
+constexpr int kItems = 4;                   // items the item warp is ahead at most
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
 constexpr int kOneTile = 5;                 // cost of a key of a one-tile item, in eighths
@@ -63,6 +64,8 @@ struct ChunkArgs {
   int batch, tokens, hq, hkv, G, T;
   int cap;                   // tokens a sequence can have in the cache
   int page_size, max_pages, num_pages, box, total_rows, slot_rows;
+  unsigned page_mul;         // floor(2^page_shift / (page_size / 8)) + 1; 0 for a contiguous cache
+  int page_shift;
   float cs;                  // scale * log2(e)
 };
 
@@ -114,16 +117,16 @@ __device__ __forceinline__ void item_shape(const ChunkArgs& a, const Seq& s, int
 }
 
 // First (b, h, item, block) of the part that starts at cost `off` inside sequence b, and that
-// sequence. Quotients and the root of the quadratic cost_before come from 64-bit floats and are
-// then put right: an integer division or a search takes thousands of cycles before a CTA's start.
+// sequence. Quotients and the root of the quadratic cost_before come from 32-bit floats and are
+// then put right: wide divisions or a search take thousands of cycles before a CTA's start.
 __device__ __forceinline__ int4 locate(const ChunkArgs& a, int b, long long off, Seq& s) {
   s = load_seq(a, b);
-  int h = (int)((double)off / (double)s.per_head);
+  int h = min((int)__fdividef((float)off, (float)s.per_head), a.hkv - 1);
   off -= h * s.per_head;
-  if (off < 0) { --h; off += s.per_head; }
-  else if (off >= s.per_head) { ++h; off -= s.per_head; }
-  const double base = (double)(max(s.len - s.n, 0) + kOver) + a.T, w = (double)a.T;
-  int i = (int)((sqrt(base * base + 4.0 * w * (double)off) - base) / (2.0 * w));
+  while (off < 0) { --h; off += s.per_head; }
+  while (off >= s.per_head) { ++h; off -= s.per_head; }
+  const float base = (float)(max(s.len - s.n, 0) + kOver + a.T), w = (float)a.T;
+  int i = (int)((__fsqrt_rn(base * base + 4.f * w * (float)off) - base) * __frcp_rn(2.f * w));
   i = min(max(i, 0), s.items - 1);
   while (i > 0 && cost_before(a, s, i) > off) --i;
   while (i + 1 < s.items && cost_before(a, s, i + 1) <= off) ++i;
@@ -146,7 +149,7 @@ __device__ __forceinline__ int4 locate(const ChunkArgs& a, int b, long long off,
   return make_int4(b, h, i, blk);
 }
 
-// The items of one CTA's part, in order; every warp role walks them by itself.
+// The items of one CTA's part, in order.
 struct Walk {
   int4 at, end;
   Seq s;
@@ -337,6 +340,8 @@ struct Shared {
   long long total;
   int4 cut[2];
   Seq first;                 // the sequence of the first cut
+  Item items[kItems];
+  uint64_t item_full[kItems], item_empty[kItems];
   float2 half_ml[kRows];     // the second warpgroup's maximum and sum (one-tile items)
 };
 
@@ -365,6 +370,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       mbar_init(&sh.o_free[i], 4);
       sh.cut[i] = make_int4(a.batch, 0, 0, 0);
     }
+    for (int i = 0; i < kItems; ++i) { mbar_init(&sh.item_full[i], 1); mbar_init(&sh.item_empty[i], 11); }
     mbar_init(&sh.half_ready, 4);
     mbar_init(&sh.teardown, kThreadsCa / 32);
     mbar_init(&sh.drain, 1);
@@ -409,7 +415,10 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   const int parts = (int)min((long long)gridDim.x, max(1ll, W / kMinWork));   // (a power of two)
   {
     const long long lo = sh.before[warp] + inc - mine;
-    const double part = (double)W / (double)parts;
+    // W / parts to 46 bits, the same in every CTA: cuts agree and ascend.
+    double inv = (double)__frcp_rn((float)parts);
+    inv = inv * (2.0 - (double)parts * inv);
+    const double part = (double)W * inv;
 #pragma unroll 1
     for (int e = 0; e < 2; ++e) {
       const int c = blockIdx.x + e;
@@ -429,10 +438,20 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     }
   }
   __syncthreads();
-  const int4 c0 = sh.cut[0], c1 = sh.cut[1];
   const uint32_t tmem = sh.tmem;
-  Walk walk(c0, c1, sh.first);
+  // The item warp walks this CTA's part and hands the items out; the other warps take a copy each
+  // (walked by every warp, the walk's state spilled, and a spilled register is an L2 access here).
   Item it;
+  int taken = 0;
+  auto next_item = [&]() -> bool {
+    const int k = taken % kItems;
+    if (sh.bail || !mbar_wait(&sh.item_full[k], (taken / kItems) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
+    it = sh.items[k];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[k]);
+    ++taken;
+    return it.b1 > 0;
+  };
 
   if (warp >= 8) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -441,16 +460,21 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     int n = 0, items = 0;                       // ring tiles issued, items
     const int pieces = kKeys / a.box;
     const uint32_t piece_bytes = (uint32_t)a.box * 256;
-    while (!sh.bail && walk.next(a, it)) {
-      // Lane p < pieces brings the p-th piece of each block; `row` is its row in the cache.
+    while (next_item()) {
+      // Lane p < pieces brings the p-th piece of each block; `row` is its row in the cache (-1: not
+      // wanted; no such page: past the end, which reads as zeros). No branches around the page
+      // loads: several are in flight.
+      const int* pages = a.pages ? a.pages + (size_t)it.b * a.max_pages : nullptr;
       auto row_of = [&](int blk) -> int {
         const int tok = blk * kKeys + lane * a.box;
-        if (blk >= it.b1 || lane >= pieces || tok >= it.kend) return -1;
-        if (a.pages == nullptr) return (it.b * a.hkv + it.h) * a.page_size + tok;
-        const int lp = tok / a.page_size;
-        const int pg = __ldcg(a.pages + (size_t)it.b * a.max_pages + lp);
-        if (pg < 0 || pg >= a.num_pages) return a.total_rows;      // no such page: zeros
-        return (pg * a.hkv + it.h) * a.page_size + (tok - lp * a.page_size);
+        const bool wanted = blk < it.b1 && lane < pieces && tok < it.kend;
+        // tok / page_size: both multiples of 8, the quotient by a product (exact below 2^28)
+        const int lp = wanted ? (int)(((unsigned long long)(unsigned)(tok >> 3) * a.page_mul) >> a.page_shift) : 0;
+        int pg = it.b;
+        if (pages) pg = __ldcg(pages + lp);
+        const int off = tok - lp * a.page_size;
+        const int row = pg < 0 || pg >= a.num_pages ? a.total_rows : (pg * a.hkv + it.h) * a.page_size + off;
+        return wanted ? row : -1;
       };
       auto issue = [&](const CUtensorMap* map, int blk, int row) -> bool {
         const int st = n % kRing;
@@ -542,7 +566,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           wait(&sh.tail, tails++, kDevTimeoutFull);
         }
       };
-      while (!failed() && !sh.bail && walk.next(a, it)) {
+      while (!failed() && next_item()) {
         wait(&sh.q_full, items++, kDevTimeoutFull);
         const int nb = it.b1 - it.b0;
         wait(&sh.full[st], ph, kDevTimeoutFull);
@@ -625,7 +649,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     // They may hold anything (a freed page's NaN): their V rows become zeros, for 0 * NaN would
     // spoil every row. The tile is the item's last in the ring; the MMA thread says when it is here.
     int n = 0, tails = 0;
-    while (!sh.bail && walk.next(a, it)) {
+    while (next_item()) {
       n += 2 * (it.b1 - it.b0);
       if (it.kend >= it.b1 * kKeys) continue;
       const int k = n - 1;
@@ -638,6 +662,21 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.tail);
+    }
+  } else {
+    // ---------------------------------------------------------- items
+    Walk walk(sh.cut[0], sh.cut[1], sh.first);
+    bool more = true;
+    for (int n = 0; more && !sh.bail; ++n) {
+      more = walk.next(a, it);
+      if (!more) it.b1 = 0;                     // no more: the last one handed out
+      const int k = n % kItems;
+      if (!mbar_wait(&sh.item_empty[k], ((n / kItems) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
+      if (lane == 0) {
+        sh.items[k] = it;
+        mbar_arrive(&sh.item_full[k]);
+      }
+      __syncwarp();
     }
   }
   } else {
@@ -652,7 +691,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     int ns = 0, no[2] = {0, 0}, nh = 0;
     if (tid < 2) a.desc[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
     named_bar_sync(1, 256);
-    while (!sh.bail && walk.next(a, it)) {
+    while (next_item()) {
       const int nb = it.b1 - it.b0;
       const int tok = it.two && slot == 1 ? a.T + rt : rt;        // token within the item
       const int vis = max(it.pos + tok + 1, 0);                    // keys this row sees
@@ -1014,6 +1053,13 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   a.cap = (int)(cap < INT_MAX - 2 * kKeys ? cap : INT_MAX - 2 * kKeys);
   a.slot_rows = slot_rows_of(tokens, G);
   a.cs = scale * kLog2eF;
+  if (page_table) {
+    const unsigned d = (unsigned)page_size / 8;
+    int log = 0;
+    while ((1u << log) < d) ++log;
+    a.page_shift = 28 + log;
+    a.page_mul = (unsigned)((1ull << a.page_shift) / d) + 1;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t prow = (size_t)2 * dev.num_sms * a.slot_rows;
   a.part_o = reinterpret_cast<float*>(ws);
