@@ -34,7 +34,7 @@ constexpr int kHd = 128;                    // head dim
 constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
 constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
 constexpr int kRing = 5;                    // K/V tiles in flight
-constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, tail, item warps
+constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, inspecting, item warps
 // Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup keeps
 // 72 (fewer and its roles spill), which lets a softmax thread hold its row of S (128 values):
 // 256 x 216 + 128 x 72 = 384 x 168.
@@ -57,6 +57,7 @@ struct ChunkArgs {
   const int32_t* cu;         // [batch + 1] first row of each sequence's new tokens
   const int32_t* lens;       // [batch] tokens in the cache, the new ones included
   const int32_t* pages;      // [batch, max_pages] or nullptr (contiguous)
+  const void *q, *k, *v;
   void* out;
   float* part_o;             // [2 * grid][32][slot_rows][4]: column fours, rows, columns
   float2* part_ml;           // [2 * grid][slot_rows] (maximum in log2 units, sum)
@@ -148,6 +149,9 @@ __device__ __forceinline__ int4 locate(const ChunkArgs& a, int b, long long off,
   }
   return make_int4(b, h, i, blk);
 }
+
+// Key block `blk` has keys that some row of the item does not see.
+__device__ __forceinline__ bool uneven(const Item& it, int blk) { return (blk + 1) * kKeys > it.pos + 1; }
 
 // The items of one CTA's part, in order.
 struct Walk {
@@ -329,9 +333,15 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The whole warp waits, and agrees on the outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
 struct Shared {
   uint64_t full[kRing], empty[kRing];
-  uint64_t q_full, q_empty, tail_go, tail;
+  uint64_t ready[kRing];
+  uint64_t q_full, q_empty;
   uint64_t s_full[2], p_full[2][2], o_full[2], o_free[2], half_ready;
   uint64_t teardown, drain;
   uint32_t tmem;
@@ -342,8 +352,67 @@ struct Shared {
   Seq first;                 // the sequence of the first cut
   Item items[kItems];
   uint64_t item_full[kItems], item_empty[kItems];
+  int odd[kItems];           // the item has a V value that is not finite and that some rows do not see
   float2 half_ml[kRows];     // the second warpgroup's maximum and sum (one-tile items)
 };
+
+// One row over the item's piece, one thread, from global memory: for items with values that are
+// not finite and that only some rows see, where a product over whole blocks cannot tell the rows
+// apart. Slow, and right: only the keys that the row sees are touched.
+template <typename T>
+__device__ __noinline__ void exact_row(const ChunkArgs& a, Item it, int tok, int rg, int vis,
+                                       T* dst, float* pdst, float2* pml) {
+  const T* q = static_cast<const T*>(a.q) + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
+  const int j0 = it.b0 * kKeys, j1 = min(vis, it.b1 * kKeys);
+  auto row_at = [&](int j) -> long long {          // -1: no such page, zeros
+    int pg = it.b, off = j;
+    if (a.pages) {
+      pg = __ldcg(a.pages + (size_t)it.b * a.max_pages + j / a.page_size);
+      off = j % a.page_size;
+      if (pg < 0 || pg >= a.num_pages) return -1;
+    }
+    return (((long long)pg * a.hkv + it.h) * a.page_size + off) * kHd;
+  };
+  auto score = [&](long long at) {
+    float s = 0.f;
+    if (at >= 0)
+      for (int d = 0; d < kHd; d += 8) {
+        float x[8], y[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(q + d), x);
+        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at + d), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
+    return s * a.cs;
+  };
+  float m = -INFINITY, l = 0.f;
+  for (int j = j0; j < j1; ++j) m = fmaxf(m, score(row_at(j)));
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int j = j0; j < j1; ++j) l += ex2(score(row_at(j)) - ref);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  for (int d = 0; d < kHd; d += 8) {
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j = j0; j < j1; ++j) {
+      const long long at = row_at(j);
+      const float p = ex2(score(at) - ref);
+      if (at < 0) continue;
+      float y[8];
+      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at + d), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(p, y[e], o[e]);
+    }
+    if (dst)
+      *reinterpret_cast<uint4*>(dst + d) =
+          make_uint4(Mma<T>::pack(o[0] * inv, o[1] * inv), Mma<T>::pack(o[2] * inv, o[3] * inv),
+                     Mma<T>::pack(o[4] * inv, o[5] * inv), Mma<T>::pack(o[6] * inv, o[7] * inv));
+    else
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<float4*>(pdst + (size_t)((d + e) / 4) * a.slot_rows * 4) =
+            make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+  }
+  if (!dst) *pml = make_float2(m, l);
+}
 
 // ------------------------------------------------------------------ the kernel
 template <typename T>
@@ -357,11 +426,9 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < kRing; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+    for (int i = 0; i < kRing; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 2); mbar_init(&sh.ready[i], 1); }
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
-    mbar_init(&sh.tail_go, 1);
-    mbar_init(&sh.tail, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i][0], 4);
@@ -445,7 +512,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   int taken = 0;
   auto next_item = [&]() -> bool {
     const int k = taken % kItems;
-    if (sh.bail || !mbar_wait(&sh.item_full[k], (taken / kItems) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
+    if (sh.bail || !warp_wait(&sh.item_full[k], (taken / kItems) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
     it = sh.items[k];
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.item_empty[k]);
@@ -478,7 +545,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       };
       auto issue = [&](const CUtensorMap* map, int blk, int row) -> bool {
         const int st = n % kRing;
-        if (!mbar_wait(&sh.empty[st], ((n / kRing) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; return false; }
+        if (!warp_wait(&sh.empty[st], ((n / kRing) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; return false; }
         const int have = min(pieces, (it.kend - blk * kKeys + a.box - 1) / a.box);
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], (uint32_t)max(have, 0) * piece_bytes);
         __syncwarp();
@@ -493,7 +560,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const int ahead = it.two ? 1 : 2;
       int r0 = row_of(it.b0), r1 = row_of(it.b0 + 1), r2 = row_of(it.b0 + 2);
       if (!issue(&a.kmap, it.b0, r0)) break;      // the ring has room before the last item's Q is free
-      if (items > 0 && !mbar_wait(&sh.q_empty, (items - 1) & 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
+      if (items > 0 && !warp_wait(&sh.q_empty, (items - 1) & 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
       if (lane == 0) {
         const uint32_t qb = (uint32_t)(a.T * a.G) * 256;
         mbar_arrive_expect_tx(&sh.q_full, it.two ? 2 * qb : qb);
@@ -524,7 +591,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const uint32_t dq = desc_kmajor(smem_u32(sq));
       const uint32_t dk = desc_kmajor(smem_u32(ring)), dv = desc_mnmajor(smem_u32(ring));
       int st = 0, ph = 0;                       // ring position
-      int items = 0, tails = 0, np0 = 0, np1 = 0, no0 = 0, no1 = 0;
+      int items = 0, np0 = 0, np1 = 0, no0 = 0, no1 = 0;
       const uint32_t one = elect_one();
       uint32_t polls = spin_limit();            // 1 once a wait has given up
       int gave_up = 0;
@@ -558,18 +625,10 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         }
         ++np;
       };
-      auto value_tile = [&](int stage, int phase, bool last) {   // V is here, its tail cleared
-        wait(&sh.full[stage], phase, kDevTimeoutFull);
-        if (last && it.kend < it.b1 * kKeys) {
-          if (one) mbar_arrive(&sh.tail_go);
-          __syncwarp();
-          wait(&sh.tail, tails++, kDevTimeoutFull);
-        }
-      };
       while (!failed() && next_item()) {
         wait(&sh.q_full, items++, kDevTimeoutFull);
         const int nb = it.b1 - it.b0;
-        wait(&sh.full[st], ph, kDevTimeoutFull);
+        wait(&sh.ready[st], ph, kDevTimeoutFull);
         score(0, st, 0);
         if (it.two) {
           // Ring order: K0 | V0 K1 | V1 K2 | ...; every tile serves both slots.
@@ -583,11 +642,11 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             advance();
             const int ks = st, kp = ph;
             if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
-            value_tile(vs, vp, last);
+            wait(&sh.ready[vs], vp, kDevTimeoutFull);
             weigh(0, vs, j == 0, np0);
             if (last) mma_commit(one, &sh.o_full[0]);
             else {
-              wait(&sh.full[ks], kp, kDevTimeoutFull);
+              wait(&sh.ready[ks], kp, kDevTimeoutFull);
               score(0, ks, 0);
             }
             if (j == 0 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
@@ -608,7 +667,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           mma_commit(one, &sh.empty[st]);
           advance();
           if (nb > 1) {
-            wait(&sh.full[st], ph, kDevTimeoutFull);
+            wait(&sh.ready[st], ph, kDevTimeoutFull);
             score(1, st, 0);
             mma_commit(one, &sh.empty[st]);
             advance();
@@ -618,14 +677,14 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             const bool odd = j & 1;
             if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
             if (j == 1 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
-            value_tile(st, ph, j + 1 == nb);
+            wait(&sh.ready[st], ph, kDevTimeoutFull);
             if (odd) weigh(1, st, j < 2, np1);
             else weigh(0, st, j < 2, np0);
             mma_commit(one, &sh.empty[st]);
             advance();
             if (j + 2 >= nb) mma_commit(one, &sh.o_full[odd]);
             else {
-              wait(&sh.full[st], ph, kDevTimeoutFull);
+              wait(&sh.ready[st], ph, kDevTimeoutFull);
               score(odd, st, 0);
               mma_commit(one, &sh.empty[st]);
               advance();
@@ -645,23 +704,51 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       mbar_wait(&sh.drain, 0, kDevTimeoutDrain);
     }
   } else if (warp == 10) {
-    // ---------------------------------------------------------- keys past the last visible one
-    // They may hold anything (a freed page's NaN): their V rows become zeros, for 0 * NaN would
-    // spoil every row. The tile is the item's last in the ring; the MMA thread says when it is here.
-    int n = 0, tails = 0;
+    // ---------------------------------------------------------- tiles looked over
+    // Every tile passes here on its way to the MMA warp, ahead of its use. A weight of 0 does not
+    // hide a value that is not finite: 0 * NaN spoils every row. Keys past the item's last
+    // visible one may hold anything (a freed page's NaN): their V rows become zeros. A later token of
+    // the chunk that is not finite is only noted, and the item's rows are done again one by one
+    // (exact_row). An exponent of ones, plus one, carries into the sign bit.
+    constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+    int n = 0;
     while (next_item()) {
-      n += 2 * (it.b1 - it.b0);
-      if (it.kend >= it.b1 * kKeys) continue;
-      const int k = n - 1;
-      if (!mbar_wait(&sh.tail_go, tails++ & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
-      uint8_t* t = ring + (k % kRing) * kTile;
-      for (int o = max(it.kend - (it.b1 - 1) * kKeys, 0) * 128 + lane * 16; o < kHalf; o += 512) {
-        *reinterpret_cast<uint4*>(t + o) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(t + kHalf + o) = make_uint4(0, 0, 0, 0);
+      const int nb = it.b1 - it.b0;
+      if (lane == 0) sh.odd[(taken - 1) % kItems] = 0;   // read after the item's last product
+      bool odd = false;
+      for (int i = 0; i < 2 * nb; ++i, ++n) {
+        const int st = n % kRing;
+        if (!warp_wait(&sh.full[st], (n / kRing) & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
+        // the tile's key block if it is a V tile, in the ring's orders (see the MMA warp)
+        const int j = it.two ? (i & 1 ? i >> 1 : -1) : (i == 2 * nb - 1 ? nb - 1 : (i >= 2 && !(i & 1) ? (i - 2) >> 1 : -1));
+        if (j >= 0 && uneven(it, it.b0 + j)) {
+          const int blk = it.b0 + j;
+          uint8_t* t = ring + st * kTile;
+          const int from = min(max(it.kend - blk * kKeys, 0), kKeys);
+          for (int o = from * 128 + lane * 16; o < kHalf; o += 512) {
+            *reinterpret_cast<uint4*>(t + o) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(t + kHalf + o) = make_uint4(0, 0, 0, 0);
+          }
+          uint32_t carry = 0;
+          auto look = [&](const uint4& x) {
+            carry |= ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
+          };
+#pragma unroll 4
+          for (int o = max(it.pos + 1 - blk * kKeys, 0) * 128 + lane * 16; o < from * 128; o += 512) {
+            look(*reinterpret_cast<const uint4*>(t + o));
+            look(*reinterpret_cast<const uint4*>(t + kHalf + o));
+          }
+          if (__any_sync(0xffffffffu, (carry & 0x80008000u) != 0)) odd = true;
+          if (odd && lane == 0) sh.odd[(taken - 1) % kItems] = 1;
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.ready[st]);
+          mbar_arrive(&sh.empty[st]);            // this warp's half of `empty`
+        }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.tail);
     }
   } else {
     // ---------------------------------------------------------- items
@@ -671,7 +758,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       more = walk.next(a, it);
       if (!more) it.b1 = 0;                     // no more: the last one handed out
       const int k = n % kItems;
-      if (!mbar_wait(&sh.item_empty[k], ((n / kItems) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
+      if (!warp_wait(&sh.item_empty[k], ((n / kItems) & 1) ^ 1, kDevTimeoutEmpty)) { sh.bail = 1; break; }
       if (lane == 0) {
         sh.items[k] = it;
         mbar_arrive(&sh.item_full[k]);
@@ -702,7 +789,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       int mine_n = 0;
       bool ok = true;
       for (int j = it.two ? 0 : slot; j < nb; j += step, ++mine_n) {
-        if (!mbar_wait(&sh.s_full[slot], ns & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
+        if (!warp_wait(&sh.s_full[slot], ns & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
         ++ns;
         fence_after();
         if (!rows) {                              // no row of this warp is in the item
@@ -796,7 +883,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       // Epilogue: O / l to the output, or O, m, l to the workspace.
       const bool joined = !it.two && nb > 1;      // slot 1 holds the odd blocks
       if (it.two || slot == 0 || joined) {
-        if (!mbar_wait(&sh.o_full[slot], no[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
+        if (!warp_wait(&sh.o_full[slot], no[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
         ++no[slot];
         fence_after();
       }
@@ -810,7 +897,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       }
       float f0 = 1.f, f1 = 0.f;
       if (joined) {
-        if (!mbar_wait(&sh.half_ready, nh & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
+        if (!warp_wait(&sh.half_ready, nh & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
         ++nh;
         fence_after();
         const float2 o = sh.half_ml[r];
@@ -830,7 +917,12 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       T* dst = out + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
       float* pdst = a.part_o + (size_t)sl * a.slot_rows * kHd + prow * 4;    // [32 column fours][rows][4]
       const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-      if (rows) {
+      const bool again = uneven(it, it.b1 - 1) && sh.odd[(taken - 1) % kItems] != 0;
+      if (again) {
+        if (live)
+          exact_row<T>(a, it, tok, rg, vis, whole ? dst : nullptr, pdst, a.part_ml + (size_t)sl * a.slot_rows + prow);
+        __syncwarp();
+      } else if (rows) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t o[32];
@@ -869,7 +961,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         }
       }
       __syncwarp();
-      if (live && !whole) a.part_ml[(size_t)sl * a.slot_rows + prow] = make_float2(m, l);
+      if (live && !whole && !again) a.part_ml[(size_t)sl * a.slot_rows + prow] = make_float2(m, l);
       fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -1044,6 +1136,7 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   if (!aligned16(workspace)) return DBK_EALIGN;
 
   ChunkArgs a{};
+  a.q = q; a.k = k_cache; a.v = v_cache;
   a.cu = cu_seqlens; a.lens = seq_lens; a.pages = page_table; a.out = out;
   a.batch = batch; a.tokens = tokens; a.hq = n_q_heads; a.hkv = n_kv_heads;
   a.G = G; a.T = kRows / G;

@@ -340,6 +340,35 @@ def test_chunk_attention_nan_stays_in_its_rows():
     assert torch.equal(out[~want_nan], clean[~want_nan])
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("ctx,new,hq,hkv", [(0, 40, 8, 2), (300, 200, 4, 4), (5000, 30, 16, 2), (90, 300, 2, 1)])
+def test_chunk_attention_later_tokens_that_are_not_finite(dt, ctx, new, hq, hkv):
+    """A V (and K) of a later token of the chunk that is not finite reaches only the rows that see it."""
+    q, k, v, cu, lens, table = make([ctx], [new], hq, hkv, 16, dt)
+    clean = ops.chunk_attention(q, k, v, cu, lens, page_table=table)
+    at = ctx + new - 7                                   # position of the seventh token from the end
+    page, off = int(table[0, at // 16]), at % 16
+    for value in (float("nan"), float("inf"), -float("inf")):
+        v2, k2 = v.clone(), k.clone()
+        v2[page, 0, off, 5] = value
+        out = ops.chunk_attention(q, k, v2, cu, lens, page_table=table)
+        group = hq // hkv
+        sees = torch.zeros(new, hq, D, dtype=torch.bool, device="cuda")
+        sees[new - 7:, :group, 5] = True
+        want = torch.full_like(out, value)
+        assert torch.equal(out[sees].isnan(), want[sees].isnan())
+        if value == value:
+            assert (out[sees] == value).all()
+        assert out[~sees].isfinite().all()
+        # the rows done one by one agree with the clean ones as two results within tolerance of one
+        check_attention(torch.where(sees, clean, out), q, k, v, [ctx], [new], table, 1 / math.sqrt(D))
+        k2[page, 0, off] = value
+        out = ops.chunk_attention(q, k2, v2, cu, lens, page_table=table)
+        assert out[:new - 7].isfinite().all()
+        check_attention(torch.cat([out[:new - 7], clean[new - 7:]]), q, k, v, [ctx], [new], table,
+                        1 / math.sqrt(D))
+
+
 def test_chunk_attention_decoding_equals_flashdecode():
     dt = torch.bfloat16
     ctx = [1, 64, 1000, 5000]
