@@ -12,7 +12,20 @@
 // running maximum and sum in fp32 registers). TMEM holds S0, S1, O0, O1 (4 x 128 columns);
 // P overwrites its own S as 16-bit pairs and is the PV product's A operand straight from TMEM.
 // An item with one tile only gives both warpgroups that tile and every other key block, and
-// merges the two halves from TMEM at its end.
+// merges the two halves from TMEM at its end. Beside the two softmax warpgroups a warp brings
+// tiles by TMA, one looks over them, one issues the MMAs, one hands out the items.
+//
+// What bounds it. A block of an item with two tiles is 2 x 2 x 128^3 products, 2,048 cycles of the
+// tensor core and 2,048 of the exponential unit; it takes ~3,000, of which a tile's softmax is
+// ~1,900: the two tiles' chains (S -> softmax -> PV -> next S) overlap but for their ends. One
+// prompt of 16,384 tokens, 32 / 8 heads: 1.72 to 1.86 ms from one GPU to another, 1.18 to 1.28
+// PFLOP/s (a plain square library product under the same power limit: 1.68 in bursts, 1.40
+// sustained). Few rows over a long cache are bound by HBM: 8 requests of one token at 16,384,
+// 64 / 8 heads: 99 us, 5.4 TB/s. Short calls pay ~9 us from launch to the first product (cold
+// code, lengths, cuts, first tiles) and ~4 for the join.
+// Measured and not kept: a share of the exponentials by polynomial on the FMA pipe (1/8: +2 %,
+// 1/2: +13 %), two issuing threads (+18 %: the tiles fall into step), no row maximum but a bound
+// from the weights' sum (+12 %), S loaded from TMEM in two halves (+10 %).
 //
 // Split. The (item, 128-key block) units of the whole batch form one line, weighted by their
 // cost; CTA c of at most one per SM takes the c-th equal part of it, whatever the lengths are
@@ -40,7 +53,9 @@ constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, i
 // 256 x 216 + 128 x 72 = 384 x 168.
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreadsCa * 168, "register split");
-constexpr int kItems = 4;                   // items the item warp is ahead at most
+// Items the item warp is ahead at most. The inspecting warp is up to four items (of one block) ahead of
+// the softmax warps that read its note `odd`, so notes are kept for more than five.
+constexpr int kItems = 8;
 constexpr int kMinBox = 8;                  // rows of the smallest TMA box
 constexpr int kOver = 256;                  // an item's fixed cost, in keys
 constexpr int kOneTile = 5;                 // cost of a key of a one-tile item, in eighths
@@ -413,6 +428,8 @@ __device__ __noinline__ void exact_row(const ChunkArgs& a, Item it, int tok, int
   }
   if (!dst) *pml = make_float2(m, l);
 }
+
+static_assert(sizeof(Shared) <= 2048, "shared memory: 227 KB less 7 tiles and the alignment");
 
 // ------------------------------------------------------------------ the kernel
 template <typename T>
@@ -1115,7 +1132,7 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
       n_q_heads % n_kv_heads != 0 || num_pages < 1 || page_size < 1)
     return DBK_ESHAPE;
   const int G = n_q_heads / n_kv_heads;
-  if (G > kRows || !(scale > 0.f) || scale > 3e38f) return DBK_ESHAPE;
+  if (G > kRows || !(scale > 0.f) || scale > 1e38f || (q && q == out)) return DBK_ESHAPE;
   const int64_t rows = (int64_t)num_pages * n_kv_heads;
   if (rows > INT_MAX || rows * page_size > INT_MAX - kKeys) return DBK_ESHAPE;
   int box = kKeys;

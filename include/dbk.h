@@ -298,8 +298,9 @@ int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* sl
  *   max_len, 128]. seq_lens are clipped to what the table holds, cu_seqlens to 0..tokens.
  *   q head h reads kv head h / (n_q_heads / n_kv_heads), any ratio up to 128. scale > 0.
  * Rows of out behind cu_seqlens[batch] are left as they were. Cache slots at and past seq_lens
- * may hold anything. Maximum, sum and output accumulate in fp32; the weights are rounded to
- * dtype for the tensor cores. Results do not depend on timing.
+ * may hold anything, and values that are not finite reach only the rows that see them. Maximum,
+ * sum and output accumulate in fp32; the weights are rounded to dtype for the tensor cores. out
+ * is not q. Results do not depend on timing.
  * workspace: dbk_chunk_attention_workspace_bytes(), need not be zero-filled, one per call that
  * may run concurrently. */
 int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,

@@ -46,7 +46,7 @@ def test_rope_append_refusals(kw, want):
 
 
 def attend(**kw):
-    a = dict(q=16, k=16, v=16, cu=16, lens=16, table=16, out=16, n=3, batch=2, hq=4, hkv=2, d=128,
+    a = dict(q=16, k=16, v=16, cu=16, lens=16, table=16, out=32, n=3, batch=2, hq=4, hkv=2, d=128,
              pages=4, page=16, width=8, scale=0.1, dt=0)
     a.update(kw)
     return N.load().dbk_chunk_attention(*[a[k] for k in (
@@ -60,7 +60,7 @@ def attend(**kw):
     (dict(batch=0), ESHAPE), (dict(page=20), ESHAPE), (dict(page=4), ESHAPE), (dict(width=0), ESHAPE),
     (dict(table=None, page=100), ESHAPE),                         # contiguous: pages != batch
     (dict(scale=0.0), ESHAPE), (dict(scale=-1.0), ESHAPE), (dict(scale=float("nan")), ESHAPE),
-    (dict(scale=float("inf")), ESHAPE), (dict(pages=1 << 24, page=128), ESHAPE),
+    (dict(scale=float("inf")), ESHAPE), (dict(scale=2e38), ESHAPE), (dict(q=32, out=32), ESHAPE), (dict(pages=1 << 24, page=128), ESHAPE),
     (dict(dt=3), EDTYPE), (dict(out=8), EALIGN), (dict(k=20), EALIGN),
     (dict(n=0, q=None, out=None), 0)])
 def test_chunk_attention_refusals(kw, want):
