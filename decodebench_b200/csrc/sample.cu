@@ -25,9 +25,9 @@
 //   draw walks 512-byte segments in index order. Each pass reads the slice again (L1 / L2).
 //
 // What bounds it. Many rows: instruction issue (62 % of the slots taken; ~200 instructions a logit, all passes
-// together). 256 rows of 128,000 fp32, top-p: 282 us,
-// 131 MB from HBM once, 0.46 TB/s, where a read alone takes 20 us. Few rows: a chain of ~30
-// barriers and the latency of each pass (one row of 128,000: 26 us). Measured and not kept: the
+// together). 256 rows of 128,000 fp32, top-p: 266 us,
+// 131 MB from HBM once, 0.49 TB/s, where a read alone takes 20 us. Few rows: a chain of ~30
+// barriers and the latency of each pass (one row of 128,000: 24 us). Measured and not kept: the
 // slice in registers over all passes (unrolled, it misses the instruction cache: slower by half),
 // 8-wide fp32 groups (306 us), a larger share of shared memory (no change).
 //
@@ -48,16 +48,17 @@ namespace cg = cooperative_groups;
 namespace dbk {
 namespace {
 
-// Threads of a CTA. Many rows (256 x 128,000 fp32: 282 us): small CTAs, four on an SM, whose phases
-// hide each other's barriers. At most two CTAs per SM: larger ones, for a slice's passes are chains of
-// dependent instructions (one row of 128,000: 26 us with 512 threads, 30 with 256, 28 with 1,024).
-constexpr int kManyThreads = 256, kFewThreads = 512, kMaxWarps = 32;
+// Threads of a CTA. Many rows (256 x 128,000 fp32: 264 us): small CTAs, three on an SM, whose phases
+// hide each other's barriers (four have 64 registers a thread, which spill: 273 us; five: 293). At
+// most one CTA per SM: larger ones, for a slice's passes are chains of dependent instructions (one
+// row of 128,000: 24 us with 512 threads; two to an SM, with 64 registers: 27).
+constexpr int kManyThreads = 256, kManyCtas = 3, kFewThreads = 512, kMaxWarps = 32;
 constexpr int kBins = 256;
 constexpr float kFine = 14.f;       // log2 distance up to which weights are 64-bit
 constexpr float kFar = 46.f;        // and past which they are nothing
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxSlice = 16384;    // logits of a CTA (the first histogram counts in 15 bits)
+constexpr int kMaxSlice = 32768;    // logits of a CTA, at most (with 256 threads 32 rounds of a warp)
 constexpr unsigned long long kNone = ~0ull;
 
 struct SampleArgs {
@@ -608,6 +609,8 @@ __global__ void __launch_bounds__(NT) sample_general_kernel(const __grid_constan
 constexpr int kCand = 256;                // members of the sub-bin the prefix ends in
 constexpr int kCoarse = 512;              // bins of the first histogram (every CTA reads all CTAs')
 constexpr int kHead = (int)(4.f * kCoarse / kFar);   // bins of the weights above 1/16
+constexpr int kParts = 2;                 // of a CTA's warps, with a histogram each: 15 bits of count
+static_assert(kMaxSlice / kParts < 1 << 15, "a part's count");
 constexpr int kSub = 64;                  // and of the second
 constexpr float kBinsPerLog2 = kCoarse / kFar;
 constexpr float kPlaces = 8.f * kCoarse - 0.5f;   // places (eighths of a bin) that count
@@ -682,11 +685,12 @@ struct Cand {
 
 template <int NT>
 struct FastShared {
-  static constexpr int kWarps = NT / 32, kList = 1280 / kWarps;       // listed logits of a warp
+  static constexpr int kWarps = NT / 32, kList = (NT == kManyThreads ? 3072 : 4096) / kWarps;   // listed logits of a warp
   static constexpr int kRounds = kMaxSlice / (4 * NT);                // rounds of vectors of a warp, at most
+  static_assert(kRounds <= 32, "a lane per round");
   Exp2Table table;
   union {
-    unsigned int coarse[kCoarse];         // count << 17 | sum of places in the bin (eighths)
+    unsigned int coarse[kParts][kCoarse]; // count << 17 | sum of places in the bin (eighths)
     Cand all[kCand];                      // later: the members of every CTA
   };
   float x[kWarps][kList];
@@ -734,7 +738,7 @@ __device__ __noinline__ bool reaches(float v, float M, float temp, float mp) {
 }
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(NT, NT == kManyThreads ? kManyCtas : 1) sample_kernel(const __grid_constant__ SampleArgs a) {
   constexpr int VN = Vec<T>::n;
   extern __shared__ double dyn[];
   using Shared = FastShared<NT>;
@@ -754,7 +758,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_cons
   const int rounds = (R.v1 - R.v0 + NT - 1) / NT;
   const int first_v = R.v0 + warp * rounds * 32 + lane;
   sh.table.fill();
-  for (int i = tid; i < kCoarse / 4; i += NT)
+  for (int i = tid; i < kParts * kCoarse / 4; i += NT)
     reinterpret_cast<uint4*>(sh.coarse)[i] = make_uint4(0, 0, 0, 0);
   if (tid < kSub) { sh.sub_mass[tid] = 0; sh.sub_count[tid] = 0; }
   if (tid < 2) sh.n_mine[tid] = 0;
@@ -849,6 +853,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_cons
   unsigned int before_lo = 0;
   if (by_k || by_p) {
     unsigned long long heavy = 0;
+    unsigned int* const hist = sh.coarse[warp * kParts / (NT / 32)];
     each_round([&](int, const float (&x)[VN]) {
       bool some = false;
 #pragma unroll
@@ -857,7 +862,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_cons
         some |= y < 8 * kHead - 0.5f;
         if (y < kPlaces) {                         // nearest place, by adding 1.5 * 2^23
           const unsigned int at = __float_as_uint(y + 12582912.f) & (8 * kCoarse - 1);
-          atomicAdd(&sh.coarse[at >> 3], (1u << 17) | (at & 7));
+          atomicAdd(&hist[at >> 3], (1u << 17) | (at & 7));
         }
       }
       if (by_p && __any_sync(0xffffffffu, some)) {
@@ -871,12 +876,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_cons
     static_assert(kCoarse / PT <= NT, "bins per thread");
     unsigned int c[PT] = {0, 0}, off[PT] = {0, 0};
     if (tid < kCoarse / PT)
-      for_cluster(C, reinterpret_cast<const uint2*>(sh.coarse) + tid, [&](int, const uint2& v) {
-        c[0] += v.x >> 17;
-        c[1] += v.y >> 17;
-        off[0] += v.x & 0x1ffff;
-        off[1] += v.y & 0x1ffff;
-      });
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+        for_cluster(C, reinterpret_cast<const uint2*>(sh.coarse[part]) + tid, [&](int, const uint2& v) {
+          c[0] += v.x >> 17;
+          c[1] += v.y >> 17;
+          off[0] += v.x & 0x1ffff;
+          off[1] += v.y & 0x1ffff;
+        });
     float f[PT], square = 0.f, near = 0.f;         // near: what the bins say of the head
     unsigned long long head_units = 0;
     if (by_p) for_cluster(C, &sh.head[0], [&](int, unsigned long long v) { head_units += v; });
@@ -953,7 +960,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const __grid_cons
     __syncthreads();
     if (by_k) {
       hi = sh.k_bin;
-      const bool whole = by_p || sh.k_count <= 8u * kList;
+      const bool whole = by_p || sh.k_count * 8 <= (unsigned int)(C * (NT / 32) * kList);
       lo = whole ? 0 : hi;
       before_lo = whole ? 0 : sh.lo_before;
     } else if (by_p) {
@@ -1259,12 +1266,15 @@ int launch_sample(const SampleArgs& a, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int VN = Vec<T>::n;
   // vectors of a row: more when rows start inside a vector
   const int nvec = a.vocab / VN + (a.vocab % VN ? 2 : 0);
-  // CTAs per row: slices of at most kMaxSlice logits. If that leaves SMs without one: large CTAs,
-  // and up to two per SM while every thread still has a vector.
+  // CTAs per row: slices of at most kMaxSlice logits, and more of them while SMs have none (few
+  // rows: large CTAs) or fewer than kManyCtas, as long as every thread still has a vector.
   int C = 1;
   while (C < kMaxCluster && (int64_t)nvec * VN > (int64_t)C * kMaxSlice) C *= 2;
-  if ((int64_t)a.batch * C > dev.num_sms) return launch_rows<T, kManyThreads>(a, dev, st, C, nvec);
-  while (C < kMaxCluster && (int64_t)a.batch * 2 * C <= 2 * dev.num_sms && nvec / (2 * C) >= kFewThreads) C *= 2;
+  if ((int64_t)a.batch * C > dev.num_sms) {
+    while (C < kMaxCluster && (int64_t)a.batch * 2 * C <= kManyCtas * dev.num_sms && nvec / (2 * C) >= kManyThreads) C *= 2;
+    return launch_rows<T, kManyThreads>(a, dev, st, C, nvec);
+  }
+  while (C < kMaxCluster && (int64_t)a.batch * 2 * C <= dev.num_sms && nvec / (2 * C) >= kFewThreads) C *= 2;
   return launch_rows<T, kFewThreads>(a, dev, st, C, nvec);
 }
 
