@@ -367,66 +367,42 @@ struct Shared {
   Seq first;                 // the sequence of the first cut
   Item items[kItems];
   uint64_t item_full[kItems], item_empty[kItems];
-  int odd[kItems];           // the item has a V value that is not finite and that some rows do not see
+  int odd[kItems];           // some V value of the item's later tokens is not finite (see add_odd)
   float2 half_ml[kRows];     // the second warpgroup's maximum and sum (one-tile items)
 };
 
-// One row over the item's piece, one thread, from global memory: for items with values that are
-// not finite and that only some rows see, where a product over whole blocks cannot tell the rows
-// apart. Slow, and right: only the keys that the row sees are touched.
+// What values of V that are not finite add to one row that sees them: the inspecting warp took those
+// of the chunk's later tokens out of the tiles (0 * Inf would reach every row), so each row adds
+// its own, from global memory, to what it has written. The weight is positive and the sum is not
+// finite whatever it is, so it counts as 1. One thread; at most 2 T keys, whatever the length.
 template <typename T>
-__device__ __noinline__ void exact_row(const ChunkArgs& a, Item it, int tok, int rg, int vis,
-                                       T* dst, float* pdst, float2* pml) {
-  const T* q = static_cast<const T*>(a.q) + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
-  const int j0 = it.b0 * kKeys, j1 = min(vis, it.b1 * kKeys);
-  auto row_at = [&](int j) -> long long {          // -1: no such page, zeros
-    int pg = it.b, off = j;
-    if (a.pages) {
-      pg = __ldcg(a.pages + (size_t)it.b * a.max_pages + j / a.page_size);
-      off = j % a.page_size;
-      if (pg < 0 || pg >= a.num_pages) return -1;
-    }
-    return (((long long)pg * a.hkv + it.h) * a.page_size + off) * kHd;
-  };
-  auto score = [&](long long at) {
-    float s = 0.f;
-    if (at >= 0)
-      for (int d = 0; d < kHd; d += 8) {
-        float x[8], y[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(q + d), x);
-        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at + d), y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
-      }
-    return s * a.cs;
-  };
-  float m = -INFINITY, l = 0.f;
-  for (int j = j0; j < j1; ++j) m = fmaxf(m, score(row_at(j)));
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int j = j0; j < j1; ++j) l += ex2(score(row_at(j)) - ref);
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+__device__ __noinline__ void add_odd(const ChunkArgs& a, Item it, int vis, float inv, T* dst, float* pdst) {
+  const int j0 = max(it.pos + 1, it.b0 * kKeys), j1 = min(vis, it.b1 * kKeys);
   for (int d = 0; d < kHd; d += 8) {
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int j = j0; j < j1; ++j) {
-      const long long at = row_at(j);
-      const float p = ex2(score(at) - ref);
-      if (at < 0) continue;
+    bool some = false;
+    for (int j = max(j0, 0); j < j1; ++j) {
+      int pg = it.b, off = j;
+      if (a.pages) {
+        pg = __ldcg(a.pages + (size_t)it.b * a.max_pages + j / a.page_size);
+        off = j % a.page_size;
+        if (pg < 0 || pg >= a.num_pages) continue;
+      }
       float y[8];
-      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at + d), y);
+      unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) +
+                                                 (((size_t)pg * a.hkv + it.h) * a.page_size + off) * kHd + d), y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = fmaf(p, y[e], o[e]);
+      for (int e = 0; e < 8; ++e)
+        if (!isfinite(y[e])) { o[e] += y[e]; some = true; }
     }
-    if (dst)
-      *reinterpret_cast<uint4*>(dst + d) =
-          make_uint4(Mma<T>::pack(o[0] * inv, o[1] * inv), Mma<T>::pack(o[2] * inv, o[3] * inv),
-                     Mma<T>::pack(o[4] * inv, o[5] * inv), Mma<T>::pack(o[6] * inv, o[7] * inv));
-    else
+    if (!some) continue;
 #pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<float4*>(pdst + (size_t)((d + e) / 4) * a.slot_rows * 4) =
-            make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    for (int e = 0; e < 8; ++e) {
+      if (o[e] == 0.f) continue;
+      if (dst) dst[d + e] = Elem<T>::from_f(Elem<T>::to_f(dst[d + e]) + o[e] * inv);
+      else pdst[(size_t)((d + e) / 4) * a.slot_rows * 4 + (d + e) % 4] += o[e];
+    }
   }
-  if (!dst) *pml = make_float2(m, l);
 }
 
 static_assert(sizeof(Shared) <= 2048, "shared memory: 227 KB less 7 tiles and the alignment");
@@ -724,16 +700,15 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     // ---------------------------------------------------------- tiles looked over
     // Every tile passes here on its way to the MMA warp, ahead of its use. A weight of 0 does not
     // hide a value that is not finite: 0 * NaN spoils every row. Keys past the item's last
-    // visible one may hold anything (a freed page's NaN): their V rows become zeros. A later token of
-    // the chunk that is not finite is only noted, and the item's rows are done again one by one
-    // (exact_row). An exponent of ones, plus one, carries into the sign bit.
+    // visible one may hold anything (a freed page's NaN): their V rows become zeros. Values of the
+    // chunk's later tokens that are not finite become zeros too and are noted: the rows that see
+    // them add them at the end (add_odd). An exponent of ones, plus one, carries into the sign bit.
     constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
     constexpr uint32_t kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
     int n = 0;
     while (next_item()) {
       const int nb = it.b1 - it.b0;
       if (lane == 0) sh.odd[(taken - 1) % kItems] = 0;   // read after the item's last product
-      bool odd = false;
       for (int i = 0; i < 2 * nb; ++i, ++n) {
         const int st = n % kRing;
         if (!warp_wait(&sh.full[st], (n / kRing) & 1, kDevTimeoutFull)) { sh.bail = 1; break; }
@@ -751,13 +726,22 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           auto look = [&](const uint4& x) {
             carry |= ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
           };
+          const int seen = max(it.pos + 1 - blk * kKeys, 0) * 128 + lane * 16;
 #pragma unroll 4
-          for (int o = max(it.pos + 1 - blk * kKeys, 0) * 128 + lane * 16; o < from * 128; o += 512) {
+          for (int o = seen; o < from * 128; o += 512) {
             look(*reinterpret_cast<const uint4*>(t + o));
             look(*reinterpret_cast<const uint4*>(t + kHalf + o));
           }
-          if (__any_sync(0xffffffffu, (carry & 0x80008000u) != 0)) odd = true;
-          if (odd && lane == 0) sh.odd[(taken - 1) % kItems] = 1;
+          if (__any_sync(0xffffffffu, (carry & 0x80008000u) != 0)) {
+            if (lane == 0) sh.odd[(taken - 1) % kItems] = 1;
+#pragma unroll 1
+            for (int o = seen; o < from * 128; o += 512)
+#pragma unroll 1
+              for (int e = 0; e < 8; ++e) {
+                uint32_t* x = reinterpret_cast<uint32_t*>(t + (e >> 2) * kHalf + o) + (e & 3);
+                *x &= ~(((((*x & kExp) + kOne) & 0x80008000u) >> 15) * 0xffffu);
+              }
+          }
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -934,12 +918,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       T* dst = out + ((size_t)(it.tok + tok) * a.hq + it.h * a.G + rg) * kHd;
       float* pdst = a.part_o + (size_t)sl * a.slot_rows * kHd + prow * 4;    // [32 column fours][rows][4]
       const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-      const bool again = uneven(it, it.b1 - 1) && sh.odd[(taken - 1) % kItems] != 0;
-      if (again) {
-        if (live)
-          exact_row<T>(a, it, tok, rg, vis, whole ? dst : nullptr, pdst, a.part_ml + (size_t)sl * a.slot_rows + prow);
-        __syncwarp();
-      } else if (rows) {
+      if (rows) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t o[32];
@@ -977,8 +956,11 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           __syncwarp();
         }
       }
+      if (uneven(it, it.b1 - 1) && sh.odd[(taken - 1) % kItems] != 0) {
+        if (live) add_odd<T>(a, it, vis, inv, whole ? dst : nullptr, pdst);
+      }
       __syncwarp();
-      if (live && !whole && !again) a.part_ml[(size_t)sl * a.slot_rows + prow] = make_float2(m, l);
+      if (live && !whole) a.part_ml[(size_t)sl * a.slot_rows + prow] = make_float2(m, l);
       fence_before();
       __syncwarp();
       if (lane == 0) {

@@ -369,6 +369,22 @@ def test_chunk_attention_later_tokens_that_are_not_finite(dt, ctx, new, hq, hkv)
                         1 / math.sqrt(D))
 
 
+def test_chunk_attention_all_values_not_finite_in_a_long_cache():
+    """Every V is NaN, or one of a long sequence's last ones: no wait runs out, all rows are right."""
+    dt = torch.bfloat16
+    q, k, v, cu, lens, table = make([40000], [700], 8, 1, 64, dt)
+    v2 = torch.full_like(v, float("nan"))
+    assert ops.chunk_attention(q, k, v2, cu, lens, page_table=table).isnan().all()
+    v2 = v.clone()
+    page = int(table[0, 40650 // 64])
+    v2[page, 0, 40650 % 64] = float("inf")
+    out = ops.chunk_attention(q, k, v2, cu, lens, page_table=table)
+    clean = ops.chunk_attention(q, k, v, cu, lens, page_table=table)
+    assert torch.equal(out[:650], clean[:650])
+    assert (out[650:] == float("inf")).all()
+    assert ops.take_device_error() == 0
+
+
 def test_chunk_attention_decoding_equals_flashdecode():
     dt = torch.bfloat16
     ctx = [1, 64, 1000, 5000]
