@@ -46,6 +46,7 @@ constexpr int kKeys = 128;                  // keys of a block (MMA N of S, K of
 constexpr int kHd = 128;                    // head dim
 constexpr int kHalf = 128 * 128;            // bytes of 128 rows x 64 16-bit values (one swizzled half)
 constexpr int kTile = 2 * kHalf;            // a Q, K or V tile
+constexpr int kMaxBatch = 65536;            // a part walks over empty sequences one by one
 constexpr int kRing = 5;                    // K/V tiles in flight
 constexpr int kThreadsCa = 384;             // 2 softmax warpgroups; TMA, MMA, inspecting, item warps
 // Registers: launched with 168 a thread (384 x 168 of the SM's 65,536); the third warpgroup keeps
@@ -1114,7 +1115,7 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
       n_q_heads % n_kv_heads != 0 || num_pages < 1 || page_size < 1)
     return DBK_ESHAPE;
   const int G = n_q_heads / n_kv_heads;
-  if (G > kRows || !(scale > 0.f) || scale > 1e38f || (q && q == out)) return DBK_ESHAPE;
+  if (G > kRows || !(scale > 0.f) || scale > 1e38f || batch > kMaxBatch) return DBK_ESHAPE;
   const int64_t rows = (int64_t)num_pages * n_kv_heads;
   if (rows > INT_MAX || rows * page_size > INT_MAX - kKeys) return DBK_ESHAPE;
   int box = kKeys;
@@ -1128,6 +1129,8 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   if (tokens == 0) return DBK_OK;
   if (!q || !out) return DBK_ENULL;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return DBK_EALIGN;
+  const size_t q_bytes = (size_t)tokens * n_q_heads * kHd * 2;
+  if (overlap(q, q_bytes, out, q_bytes)) return DBK_ESHAPE;
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;

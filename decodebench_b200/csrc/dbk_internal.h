@@ -37,6 +37,10 @@ struct PeerSet;   // comm.cuh
 int comm_peerset(const dbk_comm* c, PeerSet* ps);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
 
 // Encode a 2-D tiled TMA descriptor over a row-major [rows, inner] matrix of
 // 16-bit elements (dtype DBK_F16 / DBK_BF16), box [box_rows, box_inner], with

@@ -276,6 +276,8 @@ extern "C" int dbk_rope_append(const void* qkv, const int32_t* positions, const 
   if (!qkv || !positions || !slots || !q_out) return DBK_ENULL;
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
     return DBK_EALIGN;
+  if (overlap(qkv, (size_t)tokens * (n_q_heads + 2 * n_kv_heads) * 256, q_out, (size_t)tokens * n_q_heads * 256))
+    return DBK_ESHAPE;
   DeviceInfo dev;
   if (int rc = current_device_info(&dev)) return rc;
   RopeArgs a{};

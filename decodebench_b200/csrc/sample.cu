@@ -24,12 +24,12 @@
 //   then in the bits of the values of the bin the prefix ends in, until one value is left; the
 //   draw walks 512-byte segments in index order. Each pass reads the slice again (L1 / L2).
 //
-// What bounds it. Many rows: instruction issue (62 % of the slots taken; ~200 instructions a logit, all passes
-// together). 256 rows of 128,000 fp32, top-p: 266 us,
-// 131 MB from HBM once, 0.49 TB/s, where a read alone takes 20 us. Few rows: a chain of ~30
-// barriers and the latency of each pass (one row of 128,000: 24 us). Measured and not kept: the
-// slice in registers over all passes (unrolled, it misses the instruction cache: slower by half),
-// 8-wide fp32 groups (306 us), a larger share of shared memory (no change).
+// What bounds it. Many rows: instruction issue (62 % of the slots taken; ~200 instructions a logit,
+// all passes together). 256 rows of 128,000 fp32, top-p: 265 us, 131 MB from HBM once, 0.49 TB/s,
+// where a read alone takes 20 us. Few rows: a chain of ~30 barriers and the latency of each pass
+// (one row of 128,000: 24 us). Measured and not kept: the slice in registers over all passes
+// (unrolled, it misses the instruction cache: slower by half), 8-wide fp32 groups (8 % slower), a
+// larger share of shared memory (no change).
 //
 // Rounding. The answer is an index, and a cut that falls on another side of a sum changes it,
 // so weights and sums are wider than 32-bit floats: common path, 30-bit weights (Exp2Table) as
@@ -48,7 +48,7 @@ namespace cg = cooperative_groups;
 namespace dbk {
 namespace {
 
-// Threads of a CTA. Many rows (256 x 128,000 fp32: 264 us): small CTAs, three on an SM, whose phases
+// Threads of a CTA. Many rows (256 x 128,000 fp32: 265 us): small CTAs, three on an SM, whose phases
 // hide each other's barriers (four have 64 registers a thread, which spill: 273 us; five: 293). At
 // most one CTA per SM: larger ones, for a slice's passes are chains of dependent instructions (one
 // row of 128,000: 24 us with 512 threads; two to an SM, with 64 registers: 27).
@@ -685,7 +685,7 @@ struct Cand {
 
 template <int NT>
 struct FastShared {
-  static constexpr int kWarps = NT / 32, kList = (NT == kManyThreads ? 3072 : 4096) / kWarps;   // listed logits of a warp
+  static constexpr int kWarps = NT / 32, kList = (NT == kManyThreads ? 2048 : 4096) / kWarps;   // listed logits of a warp
   static constexpr int kRounds = kMaxSlice / (4 * NT);                // rounds of vectors of a warp, at most
   static_assert(kRounds <= 32, "a lane per round");
   Exp2Table table;
@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(NT, NT == kManyThreads ? kManyCtas : 1) sample
   const Row R = load_row<T>(a);
   const bool greedy = !(R.temp > 0.f);
 
-  // Warp w has the w-th contiguous sixteenth of the slice, in 512-byte rounds of its lanes, so
+  // Warp w has the w-th contiguous part of the slice, in 512-byte rounds of its lanes, so
   // warp, round, lane, element is index order.
   // (Loops over the rounds are not unrolled: straight-line code for a slice is several times the
   // instruction cache, and took 5 to 10 times as long.)

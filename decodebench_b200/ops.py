@@ -630,7 +630,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with p < 0 gives zeros. Chunks of any length, of 0 and of 1 token included. Paged caches
     (``page_table`` int32 [batch, max_pages]): k/v [pages, Hkv, page_size, 128], page_size a
     multiple of 8; contiguous: [batch, Hkv, max_len, 128]. ``scale`` (> 0) defaults to
-    1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` (not q itself) are left as they were."""
+    1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` (which must not overlap q) are left as they were."""
     dev = (_cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens) if page_table is None else
            _cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens, page_table))
     _check_out(out, dev)

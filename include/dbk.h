@@ -280,7 +280,7 @@ int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_
  *   inv_freq[i], formed in 64 bits); q -> q_out [tokens, n_q_heads, 128]; k, v -> slot slots[t] of
  *   k_cache, v_cache [num_pages, n_kv_heads, page_size, 128] (a contiguous cache [batch,
  *   n_kv_heads, max_len, 128] is one page per sequence: slot = b * max_len + position).
- * A slot outside the cache (-1 for a padded row) writes q only. Slots must differ from one
+ * q_out does not overlap qkv. A slot outside the cache (-1 for a padded row) writes q only. Slots must differ from one
  * another; of two rows with one slot either may be kept, in parts. head_dim 128 only. */
 int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* slots,
                     const float* inv_freq, void* q_out, void* k_cache, void* v_cache, int tokens,
@@ -300,7 +300,7 @@ int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* sl
  * Rows of out behind cu_seqlens[batch] are left as they were. Cache slots at and past seq_lens
  * may hold anything, and values that are not finite reach only the rows that see them. Maximum,
  * sum and output accumulate in fp32; the weights are rounded to dtype for the tensor cores. out
- * is not q. Results do not depend on timing.
+ * does not overlap q; batch <= 65536. Results do not depend on timing.
  * workspace: dbk_chunk_attention_workspace_bytes(), need not be zero-filled, one per call that
  * may run concurrently. */
 int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,

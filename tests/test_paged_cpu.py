@@ -40,7 +40,7 @@ def append(**kw):
 @pytest.mark.parametrize("kw,want", [
     (dict(qkv=None), ENULL), (dict(inv=None), ENULL), (dict(k=None), ENULL), (dict(d=64), ESHAPE),
     (dict(n=-1), ESHAPE), (dict(hq=0), ESHAPE), (dict(page=0), ESHAPE), (dict(dt=2), EDTYPE),
-    (dict(q=24), EALIGN), (dict(v=8), EALIGN), (dict(n=0, qkv=None, q=None), 0)])
+    (dict(q=24), EALIGN), (dict(v=8), EALIGN), (dict(q=16), ESHAPE), (dict(q=16 + 3 * 8 * 256 - 16), ESHAPE), (dict(n=0, qkv=None, q=None), 0)])
 def test_rope_append_refusals(kw, want):
     assert append(**kw) == want
 
@@ -60,7 +60,8 @@ def attend(**kw):
     (dict(batch=0), ESHAPE), (dict(page=20), ESHAPE), (dict(page=4), ESHAPE), (dict(width=0), ESHAPE),
     (dict(table=None, page=100), ESHAPE),                         # contiguous: pages != batch
     (dict(scale=0.0), ESHAPE), (dict(scale=-1.0), ESHAPE), (dict(scale=float("nan")), ESHAPE),
-    (dict(scale=float("inf")), ESHAPE), (dict(scale=2e38), ESHAPE), (dict(q=32, out=32), ESHAPE), (dict(pages=1 << 24, page=128), ESHAPE),
+    (dict(scale=float("inf")), ESHAPE), (dict(scale=2e38), ESHAPE),
+    (dict(out=16), ESHAPE), (dict(out=16 + 3 * 4 * 256 - 16), ESHAPE), (dict(batch=65537), ESHAPE), (dict(pages=1 << 24, page=128), ESHAPE),
     (dict(dt=3), EDTYPE), (dict(out=8), EALIGN), (dict(k=20), EALIGN),
     (dict(n=0, q=None, out=None), 0)])
 def test_chunk_attention_refusals(kw, want):
