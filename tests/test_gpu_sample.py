@@ -104,6 +104,34 @@ def test_flat_and_long_tails(dt):
         check(x, u, **f)
 
 
+@pytest.mark.parametrize("dt,vocab", [(F32, 32768), (F32, 32771), (BF16, 32768), (F16, 32761)])
+def test_many_rows_with_the_largest_slices(dt, vocab):
+    """More rows than SMs: a CTA has up to 32,768 logits, here also all in one bin of its histogram."""
+    batch = 160
+    x, u = rows(batch, vocab, dt, 11)
+    for b in range(0, batch, 8):               # all but one alike, at several places of a bin
+        x[b] = 0.0
+        x[b, (b * 977) % vocab] = 1.0 + b / 64
+    for b in range(1, batch, 8):               # a few values, many of each
+        x[b] = torch.randint(-3, 4, (vocab,), generator=torch.Generator().manual_seed(b)).to(dt)
+    check(x, u, top_p=0.9, temperature=0.7)
+    check(x, u, top_k=1000, top_p=0.95)
+    k = torch.tensor([1, 40, 5000, vocab - 1], dtype=torch.int32).repeat(batch // 4)
+    check(x, u, top_k=k)
+    check(x, u, min_p=0.05)
+
+
+@pytest.mark.parametrize("dt,batch,vocab", [(F32, 2, 300001), (BF16, 3, 262145), (F16, 1, 1 << 20), (F32, 150, 262148)])
+def test_vocabularies_past_a_cluster_of_slices(dt, batch, vocab):
+    x, u = rows(batch, vocab, dt, 12)
+    check(x, u, top_p=0.9, temperature=0.7)
+    if batch < 10:
+        check(x, u, top_k=1000, top_p=0.95)
+        check(x, u, top_k=50)
+        check(x, u, min_p=0.05)
+        check(x, u)
+
+
 def test_ties():
     """Equal logits: the lower index comes first in every cut."""
     u = torch.tensor([0.0, 0.3, 0.6, 0.999999])
