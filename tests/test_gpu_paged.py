@@ -303,6 +303,25 @@ def test_chunk_attention_rows_that_see_nothing_and_rows_behind():
     assert (out[:60] == 0).all() and (out[60:] == 9.0).all()
 
 
+def test_chunk_attention_batches_that_are_mostly_empty():
+    dt = torch.float16
+    q, k, v, _, _, table = make([300, 20, 700], [5, 0, 140], 8, 2, 16, dt)
+    clean = ops.chunk_attention(q, k, v, i32([0, 5, 5, 145]), i32([305, 20, 840]), page_table=table)
+    batch, at = 20000, (7, 12000, 19998)                   # the three among many without a new token
+    new, lens = torch.zeros(batch, dtype=torch.int32), torch.full((batch,), 33, dtype=torch.int32)
+    many = torch.full((batch, table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    for i, b in enumerate(at):
+        new[b], lens[b], many[b] = (5, 0, 140)[i], (305, 20, 840)[i], table[i]
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32), new.cumsum(0).int()])
+    out = ops.chunk_attention(q, k, v, cu.cuda(), lens.cuda(), page_table=many)
+    check_attention(out[:5], q[:5], k, v, [300], [5], table[:1], 1 / math.sqrt(D))
+    check_attention(out[5:], q[5:], k, v, [700], [140], table[2:], 1 / math.sqrt(D))
+    check_attention(clean[5:], q[5:], k, v, [700], [140], table[2:], 1 / math.sqrt(D))
+    out = torch.full_like(q, 9.0)                           # and none at all
+    ops.chunk_attention(q, k, v, torch.zeros_like(cu, device="cuda"), lens.cuda(), page_table=many, out=out)
+    assert (out == 9.0).all() and ops.take_device_error() == 0
+
+
 def test_chunk_attention_bad_pages_read_as_zeros():
     dt = torch.float16
     q, k, v, cu, lens, table = make([100], [30], 4, 2, 16, dt)
