@@ -25,9 +25,9 @@
 //   draw walks 512-byte segments in index order. Each pass reads the slice again (L1 / L2).
 //
 // What bounds it. Many rows: dependent instructions (~120 a logit, all passes together; half of the
-// issue slots taken by 24 warps on an SM) and the barriers between passes. 256 rows of 128,000 fp32, top-p: 265 us, 131 MB from HBM once, 0.49 TB/s,
-// where a read alone takes 20 us. Few rows: a chain of ~30 barriers and the latency of each pass
-// (one row of 128,000: 24 us). Measured and not kept: the slice in registers over all passes
+// issue slots taken by 24 warps on an SM) and the barriers between passes. 256 rows of 128,000 fp32,
+// top-p: 265 us, 131 MB from HBM once, 0.49 TB/s, where a read alone takes 20 us. Few rows: a chain of
+// ~30 barriers and the latency of each pass (one row of 128,000: 24 us). Measured and not kept: the slice in registers over all passes
 // (unrolled, it misses the instruction cache: slower by half), 8-wide fp32 groups (8 % slower), a
 // larger share of shared memory (no change).
 //
