@@ -65,7 +65,6 @@ constexpr long long kMinWork = 1024;        // least work of a CTA, in keys
 // Neighbouring cuts are at least kMinWork apart and move by less than half of that, so no part
 // between two others is empty (the join walks the parts of an item one by one).
 static_assert(kMinWork > kOver + (2 * kSnap + 1) * 128, "cuts could meet");
-constexpr float kGrow = 8.f;                // log2 growth of the maximum that forces a rescale
 constexpr float kLog2eF = 1.4426950408889634f;
 
 struct ChunkArgs {
@@ -349,6 +348,15 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// kGrow: log2 growth of a row's maximum over the one in use that forces a rescale; kBias: log2 of the
+// weight at the maximum in use. fp16 has no value between 0 and 2^-24, and l counts what P V then
+// lacks (30,000 equal keys 17 nats below a sink whose v is 0, with weights up to 2^8: 14 times the
+// half step of a rounded weight off). Here weights reach up to 2^15, so that those down to 2^-25 of the
+// largest have all 11 bits and the others are off by 2^-36 of it at most. Sums, O and partials
+// scale alike. A rescale at 2^4 instead of 2^8 costs nothing measurable.
+template <typename T> constexpr float kGrow = std::is_same<T, __nv_bfloat16>::value ? 8.f : 4.f;
+template <typename T> constexpr float kBias = std::is_same<T, __nv_bfloat16>::value ? 0.f : 11.f;
+
 // The whole warp waits, and agrees on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
@@ -816,8 +824,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         // The weights of the first 64 keys are formed with the maximum of the blocks before while
         // the row's maximum is still being found (the exponential unit is what they wait for). Only
         // if a row's maximum grew by more than kGrow (in log2 units) are they formed again and
-        // O is rescaled: weights stay below 2^kGrow, in range for 16 bits, and a lagging
-        // reference costs a floating-point weight no precision.
+        // O is rescaled: weights stay below 2^(kGrow + kBias), in range for 16 bits.
         auto weights = [&](int hf, float nm, uint32_t (&p)[32], f2 (&sum)[2]) {
           const f2 cs2 = f2_make(a.cs, a.cs), nm2 = f2_make(nm, nm);
 #pragma unroll
@@ -848,12 +855,13 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot][hf]);
         };
+        auto offset = [&]() { return m == -INFINITY ? 0.f : kBias<T> - m; };
         if (mine_n == 0) m = row_max();
         uint32_t p[32];
         f2 sum[2] = {0, 0};
-        weights(0, m == -INFINITY ? 0.f : -m, p, sum);
+        weights(0, offset(), p, sum);
         const float top = row_max();
-        const bool grow = top > m + kGrow;
+        const bool grow = top > m + kGrow<T>;
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? top : m;
           const float f = grow ? ex2(m - mn) : 1.f;               // m = -inf: 0
@@ -871,10 +879,10 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           l *= f;
           m = mn;
           sum[0] = sum[1] = 0;
-          weights(0, m == -INFINITY ? 0.f : -m, p, sum);
+          weights(0, offset(), p, sum);
         }
         publish(0, p);
-        weights(1, m == -INFINITY ? 0.f : -m, p, sum);
+        weights(1, offset(), p, sum);
         publish(1, p);
         float l0, l1;
         f2_split(f2_add(sum[0], sum[1]), l0, l1);
