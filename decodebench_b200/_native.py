@@ -13,6 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libdbk.so"
 
 DBK_F16, DBK_BF16, DBK_F32 = 0, 1, 2
+DBK_WEIGHTS_ONE = 0x100
 DBK_ESHAPE = -2
 DBK_OP_RMSNORM_GEMV, DBK_OP_GATEUP_SWIGLU, DBK_OP_GEMV = 0, 1, 2
 

@@ -10,18 +10,23 @@
 // S = Q K^T and O += P V of both run on tcgen05 with M = N = 128, and while the tensor cores
 // work on one tile the other tile's softmax runs (one warpgroup per tile, one thread per row,
 // running maximum and sum in fp32 registers). TMEM holds S0, S1, O0, O1 (4 x 128 columns);
-// P overwrites its own S as 16-bit pairs and is the PV product's A operand straight from TMEM.
+// P overwrites its own S as 16-bit pairs (high parts in the first 64 columns, low parts behind them)
+// and is the PV product's A operand straight from TMEM.
 // An item with one tile only gives both warpgroups that tile and every other key block, and
 // merges the two halves from TMEM at its end. Beside the two softmax warpgroups a warp brings
 // tiles by TMA, one looks over them, one issues the MMAs, one hands out the items.
 //
-// What bounds it. A block of an item with two tiles is 2 x 2 x 128^3 products, 2,048 cycles of the
-// tensor core and 2,048 of the exponential unit; it takes ~3,000, of which a tile's softmax is
-// ~1,900: the two tiles' chains (S -> softmax -> PV -> next S) overlap but for their ends. One
-// prompt of 16,384 tokens, 32 / 8 heads: 1.72 to 1.86 ms from one GPU to another, 1.18 to 1.28
-// PFLOP/s (a plain square library product under the same power limit: 1.68 in bursts, 1.40
-// sustained). Few rows over a long cache are bound by HBM: 8 requests of one token at 16,384,
-// 64 / 8 heads: 99 us, 5.4 TB/s. Short calls pay ~9 us from launch to the first product (cold
+// Weights. Each goes to the tensor cores as the sum of two 16-bit values, so that the result's
+// rounding is the only one of its size (root-mean-square error against 64 bits: that of a result
+// rounded once, to four digits); as one value it is 1.3 times that, and faster (below: "one part").
+//
+// What bounds it. A block of an item with two tiles is 2 x 3 x 128^3 products, 3,072 cycles of the
+// tensor core, and 2,048 of the exponential unit; it takes ~4,100 (one part: 2,048, ~3,000): the two
+// tiles' chains (S -> softmax -> PV -> next S) overlap but for their ends. One prompt of 16,384
+// tokens, 32 / 8 heads: 2.48 to 2.63 ms from one GPU to another (one part: 1.72 to 1.90), 1.25 to 1.33
+// PFLOP/s of issued products (a plain square library product under the same power limit: 1.68 in
+// bursts, 1.40 sustained). Few rows over a long cache are bound by HBM: 8 requests of one token at
+// 16,384, 64 / 8 heads: 102 us, 5.2 TB/s. Short calls pay ~9 us from launch to the first product (cold
 // code, lengths, cuts, first tiles) and ~4 for the join.
 // Measured and not kept: a share of the exponentials by polynomial on the FMA pipe (1/8: +2 %,
 // 1/2: +13 %), two issuing threads (+18 %: the tiles fall into step), no row maximum but a bound
@@ -286,23 +291,21 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
       "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
       : DBK_R8(v, 0), DBK_R8(v, 8), DBK_R8(v, 16), DBK_R8(v, 24) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8), DBK_I8(v, 16), DBK_I8(v, 24) : "memory");
-}
 __device__ __forceinline__ void tmem_ld16u(uint32_t addr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
       "%15}, [%16];"
       : DBK_R8(v, 0), DBK_R8(v, 8) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st16u(uint32_t addr, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
       "%14,%15,%16};"
       ::"r"(addr), DBK_I8(v, 0), DBK_I8(v, 8) : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(addr), DBK_I8(v, 0) : "memory");
 }
 // Waits for this thread's TMEM loads; the values pass through it, so no use can move before it.
 #define DBK_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), \
@@ -347,6 +350,25 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   f2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// A weight as the sum of two 16-bit values, a pair of keys at a time: its leading bits (8 in bf16, 11
+// in fp16), cut off, and the rest, rounded: 2^-16 of the weight are left, or 2^-22 (in fp16 no
+// less than 2^-25 of 1). 2^-24 of the weight is added to the rest, for 0 * Inf is NaN: the low part
+// of a weight must not be 0 where a row sees an infinite V.
+template <typename T>
+__device__ __forceinline__ uint32_t high_parts(float x0, float x1) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) r = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+  else asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x1), "f"(x0));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t low_parts(float x0, float x1) {
+  constexpr uint32_t kLead = std::is_same<T, __nv_bfloat16>::value ? 0xffff0000u : 0xffffe000u;
+  constexpr float kLess = -(1.f - 0x1p-24f);
+  const f2 h = f2_make(__uint_as_float(__float_as_uint(x0) & kLead), __uint_as_float(__float_as_uint(x1) & kLead));
+  f2_split(f2_fma(h, f2_make(kLess, kLess), f2_make(x0, x1)), x0, x1);
+  return Mma<T>::pack(x0, x1);
 }
 // kGrow: log2 growth of a row's maximum over the one in use that forces a rescale; kBias: log2 of the
 // weight at the maximum in use. fp16 has no value between 0 and 2^-24, and l counts what P V then
@@ -417,7 +439,7 @@ __device__ __noinline__ void add_odd(const ChunkArgs& a, Item it, int vis, float
 static_assert(sizeof(Shared) <= 2048, "shared memory: 227 KB less 7 tiles and the alignment");
 
 // ------------------------------------------------------------------ the kernel
-template <typename T>
+template <typename T, bool kTwo>
 __global__ void __launch_bounds__(kThreadsCa, 1)
 chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -512,14 +534,21 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
   // (walked by every warp, the walk's state spilled, and a spilled register is an L2 access here).
   Item it;
   int taken = 0;
-  auto next_item = [&]() -> bool {
+  auto take_item = [&]() -> bool {
     const int k = taken % kItems;
     if (sh.bail || !warp_wait(&sh.item_full[k], (taken / kItems) & 1, kDevTimeoutFull)) { sh.bail = 1; return false; }
     it = sh.items[k];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.item_empty[k]);
     ++taken;
     return it.b1 > 0;
+  };
+  auto give_back = [&]() {                      // the item last taken is not read any more
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[(taken - 1) % kItems]);
+  };
+  auto next_item = [&]() -> bool {
+    const bool some = take_item();
+    if (some) give_back();
+    return some;
   };
 
   if (warp >= 8) {
@@ -593,7 +622,10 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
       const uint32_t dq = desc_kmajor(smem_u32(sq));
       const uint32_t dk = desc_kmajor(smem_u32(ring)), dv = desc_mnmajor(smem_u32(ring));
       int st = 0, ph = 0;                       // ring position
-      int items = 0, np0 = 0, np1 = 0, no0 = 0, no1 = 0;
+      // Parities of what has been waited for, a bit each: weights and O of slot 0 and 1, Q (one register).
+      // A wait for the other parity of a barrier that nobody has arrived at yet passes.
+      constexpr uint32_t kP = 1, kO = 4, kQ = 16;
+      uint32_t par = 0;
       const uint32_t one = elect_one();
       uint32_t polls = spin_limit();            // 1 once a wait has given up
       int gave_up = 0;
@@ -614,21 +646,30 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         }
         mma_commit(one, &sh.s_full[slot]);
       };
-      // O[slot] (+)= P[slot] V, each half of the keys as soon as its weights are there.
-      auto weigh = [&](int slot, int stage, bool first, int& np) {
+      // O[slot] (+)= P[slot] V: the high parts of each half of the keys as soon as they are there,
+      // then the low parts. (Addresses formed ahead of the loop would be spilled: the compiler
+      // is kept from knowing that `ta` is the same every time.)
+      auto weigh = [&](int slot, int stage, bool first) {
         const uint32_t b0 = dv + stage * (kTile >> 4);
+        uint32_t ta = tmem + slot * 128;
+        asm volatile("" : "+r"(ta));
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          wait(&sh.p_full[slot][hf], np, kDevTimeoutMma);
+          wait(&sh.p_full[slot][hf], (par >> slot) & 1, kDevTimeoutMma);
 #pragma unroll
-          for (int s = 4 * hf; s < 4 * hf + 4; ++s)
-            mma_ts(one, tmem + 256 + slot * 128, tmem + slot * 128 + s * 8, b0 + s * (2048 >> 4), id_o,
-                   (first && s == 0) ? 0u : 1u);
+          for (int lo = 0; lo < (kTwo ? 2 : 1); ++lo)
+#pragma unroll
+            for (int s = 4 * hf; s < 4 * hf + 4; ++s)
+              mma_ts(one, ta + 256, ta + lo * 64 + s * 8, b0 + s * (2048 >> 4), id_o,
+                     (first && lo == 0 && s == 0) ? 0u : 1u);
         }
-        ++np;
+        par ^= kP << slot;
       };
+      // O[slot] of the item before has been read.
+      auto o_free = [&](int slot) { wait(&sh.o_free[slot], ((par >> (2 + slot)) & 1) ^ 1, kDevTimeoutMma); };
       while (!failed() && next_item()) {
-        wait(&sh.q_full, items++, kDevTimeoutFull);
+        wait(&sh.q_full, (par >> 4) & 1, kDevTimeoutFull);
+        par ^= kQ;
         const int nb = it.b1 - it.b0;
         wait(&sh.ready[st], ph, kDevTimeoutFull);
         score(0, st, 0);
@@ -643,16 +684,16 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
             const bool last = j + 1 == nb;
             advance();
             const int ks = st, kp = ph;
-            if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
+            if (j == 0) o_free(0);
             wait(&sh.ready[vs], vp, kDevTimeoutFull);
-            weigh(0, vs, j == 0, np0);
+            weigh(0, vs, j == 0);
             if (last) mma_commit(one, &sh.o_full[0]);
             else {
               wait(&sh.ready[ks], kp, kDevTimeoutFull);
               score(0, ks, 0);
             }
-            if (j == 0 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
-            weigh(1, vs, j == 0, np1);
+            if (j == 0) o_free(1);
+            weigh(1, vs, j == 0);
             mma_commit(one, &sh.empty[vs]);
             if (last) mma_commit(one, &sh.o_full[1]);
             else {
@@ -662,8 +703,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               if (j + 2 == nb) mma_commit(one, &sh.q_empty);
             }
           }
-          ++no0;
-          ++no1;
+          par ^= kO | (kO << 1);
         } else {
           // Ring order: K0 K1 | V0 K2 | V1 K3 | ...; block j belongs to slot j & 1.
           mma_commit(one, &sh.empty[st]);
@@ -677,11 +717,11 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           if (nb <= 2) mma_commit(one, &sh.q_empty);
           for (int j = 0; j < nb && !failed(); ++j) {
             const bool odd = j & 1;
-            if (j == 0 && no0 > 0) wait(&sh.o_free[0], no0 - 1, kDevTimeoutMma);
-            if (j == 1 && no1 > 0) wait(&sh.o_free[1], no1 - 1, kDevTimeoutMma);
+            if (j == 0) o_free(0);
+            if (j == 1) o_free(1);
             wait(&sh.ready[st], ph, kDevTimeoutFull);
-            if (odd) weigh(1, st, j < 2, np1);
-            else weigh(0, st, j < 2, np0);
+            if (odd) weigh(1, st, j < 2);
+            else weigh(0, st, j < 2);
             mma_commit(one, &sh.empty[st]);
             advance();
             if (j + 2 >= nb) mma_commit(one, &sh.o_full[odd]);
@@ -693,8 +733,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               if (j + 3 == nb) mma_commit(one, &sh.q_empty);
             }
           }
-          ++no0;
-          if (nb > 1) ++no1;
+          par ^= nb > 1 ? kO | (kO << 1) : kO;
         }
       }
       if (gave_up) {
@@ -788,17 +827,18 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
     int ns = 0, no[2] = {0, 0}, nh = 0;
     if (tid < 2) a.desc[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
     named_bar_sync(1, 256);
-    while (next_item()) {
+    while (take_item()) {
       const int nb = it.b1 - it.b0;
       const int tok = it.two && slot == 1 ? a.T + rt : rt;        // token within the item
       const int vis = max(it.pos + tok + 1, 0);                    // keys this row sees
+      const int ahead = vis - it.b0 * kKeys;                       // of them from the piece's first key on
       const int step = it.two ? 1 : 2;
       const bool live = r < a.T * a.G && tok < it.ntok;
       const bool rows = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
       int mine_n = 0;
       bool ok = true;
-      for (int j = it.two ? 0 : slot; j < nb; j += step, ++mine_n) {
+      for (int j = step == 1 ? 0 : slot; j < nb; j += step, ++mine_n) {
         if (!warp_wait(&sh.s_full[slot], ns & 1, kDevTimeoutMma)) { sh.bail = 1; ok = false; break; }
         ++ns;
         fence_after();
@@ -812,7 +852,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         for (int q = 0; q < 4; ++q) tmem_ld32(t_s + q * 32, s[q]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_wait_ld(s[q]);
-        const int lim = vis - (it.b0 + j) * kKeys;                 // keys this row sees of the block
+        const int lim = ahead - j * kKeys;                         // keys this row sees of the block
         if (lim < kKeys) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -821,46 +861,58 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               if (q * 32 + c >= lim) s[q][c] = 0xff800000u;        // -inf
         }
         __syncwarp();
-        // The weights of the first 64 keys are formed with the maximum of the blocks before while
-        // the row's maximum is still being found (the exponential unit is what they wait for). Only
-        // if a row's maximum grew by more than kGrow (in log2 units) are they formed again and
-        // O is rescaled: weights stay below 2^(kGrow + kBias), in range for 16 bits.
-        auto weights = [&](int hf, float nm, uint32_t (&p)[32], f2 (&sum)[2]) {
+        // The weights of the first 64 keys are formed, and put in place of their scores, with the
+        // maximum of the blocks before while the row's maximum is still being found (the exponential
+        // unit is what they wait for). Only if a row's maximum grew by more than kGrow (in log2 units) are
+        // they formed again and O is rescaled: weights stay below 2^(kGrow + kBias), in range for
+        // 16 bits. Measured and not kept: low parts formed behind all the high ones, while the tensor
+        // core works on those, with a barrier of their own (+4 %), or two (+7 %).
+        constexpr int kG = kTwo ? 8 : 16;        // pairs stored at a time (16 spill with two parts, 8 with one)
+        auto weights = [&](int hf, float nm, f2 (&sum)[2]) {
           const f2 cs2 = f2_make(a.cs, a.cs), nm2 = f2_make(nm, nm);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const int q = hf * 2 + (c >> 4), e = (2 * c) & 31;
-            const f2 x = f2_fma(f2_make(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), cs2, nm2);
-            float x0, x1;
-            f2_split(x, x0, x1);
-            x0 = ex2(x0);
-            x1 = ex2(x1);
-            sum[c & 1] = f2_add(sum[c & 1], f2_make(x0, x1));
-            p[c] = Mma<T>::pack(x0, x1);
+          for (int c0 = 0; c0 < 32; c0 += kG) {
+            uint32_t hi[kG], lo[kG];
+#pragma unroll
+            for (int c = c0; c < c0 + kG; ++c) {
+              const int q = hf * 2 + (c >> 4), e = (2 * c) & 31;
+              const f2 x = f2_fma(f2_make(__uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1])), cs2, nm2);
+              float x0, x1;
+              f2_split(x, x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              sum[c & 1] = f2_add(sum[c & 1], f2_make(x0, x1));
+              if (kTwo) {
+                hi[c - c0] = high_parts<T>(x0, x1);
+                lo[c - c0] = low_parts<T>(x0, x1);
+              } else {
+                hi[c - c0] = Mma<T>::pack(x0, x1);
+              }
+            }
+            tmem_st(t_s + hf * 32 + c0, hi);
+            if (kTwo) tmem_st(t_s + 64 + hf * 32 + c0, lo);
           }
         };
-        auto row_max = [&]() {
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 32; c += 2)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(s[q][c])), __uint_as_float(s[q][c + 1]));
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.cs;
-        };
-        auto publish = [&](int hf, const uint32_t (&p)[32]) {
-          tmem_st32(t_s + hf * 32, p);
+        auto publish = [&](int hf) {
           tmem_wait_st();
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[slot][hf]);
         };
         auto offset = [&]() { return m == -INFINITY ? 0.f : kBias<T> - m; };
-        if (mine_n == 0) m = row_max();
-        uint32_t p[32];
+        float top;
+        {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 32; c += 2)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(s[q][c])), __uint_as_float(s[q][c + 1]));
+          top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.cs;
+        }
+        if (mine_n == 0) m = top;
         f2 sum[2] = {0, 0};
-        weights(0, offset(), p, sum);
-        const float top = row_max();
+        weights(0, offset(), sum);
         const bool grow = top > m + kGrow<T>;
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? top : m;
@@ -873,24 +925,27 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
               tmem_wait_ld(o);
 #pragma unroll
               for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-              tmem_st16u(t_o + slot * 128 + q * 16, o);
+              tmem_st(t_o + slot * 128 + q * 16, o);
             }
           }
           l *= f;
           m = mn;
           sum[0] = sum[1] = 0;
-          weights(0, offset(), p, sum);
+          tmem_wait_st();
+          weights(0, offset(), sum);
         }
-        publish(0, p);
-        weights(1, offset(), p, sum);
-        publish(1, p);
+        publish(0);
+        weights(1, offset(), sum);
+        publish(1);
         float l0, l1;
         f2_split(f2_add(sum[0], sum[1]), l0, l1);
         l += l0 + l1;
       }
       if (!ok) break;
 
-      // Epilogue: O / l to the output, or O, m, l to the workspace.
+      // Epilogue: O / l to the output, or O, m, l to the workspace. (The item is read again: its
+      // registers are wanted in the loop.)
+      it = sh.items[(taken - 1) % kItems];
       const bool joined = !it.two && nb > 1;      // slot 1 holds the odd blocks
       if (it.two || slot == 0 || joined) {
         if (!warp_wait(&sh.o_full[slot], no[slot] & 1, kDevTimeoutMma)) { sh.bail = 1; break; }
@@ -903,6 +958,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.half_ready);
         }
+        give_back();
         continue;
       }
       float f0 = 1.f, f1 = 0.f;
@@ -976,6 +1032,7 @@ chunk_attention_kernel(const __grid_constant__ ChunkArgs a) {
         mbar_arrive(&sh.o_free[slot]);
         if (joined) mbar_arrive(&sh.o_free[1]);
       }
+      give_back();
     }
   }
   // Teardown: every warp arrives once; the MMA warp frees TMEM when all have.
@@ -1073,10 +1130,10 @@ size_t ws_bytes_of(int sms, int64_t tokens, int G) {
   return rows * (kHd * sizeof(float) + sizeof(float2)) + (size_t)2 * sms * sizeof(int4) + 256;
 }
 
-template <typename T>
+template <typename T, bool kTwo>
 int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
   const size_t smem = 1024 + (size_t)(2 + kRing) * kTile + sizeof(Shared);
-  const void* kern = reinterpret_cast<const void*>(&chunk_attention_kernel<T>);
+  const void* kern = reinterpret_cast<const void*>(&chunk_attention_kernel<T, kTwo>);
   if (int rc = allow_dynamic_smem(kern, dev, smem)) return rc;
   if (int rc = launch_pdl(kern, dim3(dev.num_sms), dim3(kThreadsCa), smem, st, &a)) return rc;
   const unsigned y = (a.slot_rows + kJoinRows - 1) / kJoinRows;
@@ -1118,6 +1175,8 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
                                    int page_size, int max_pages_per_seq, float scale, int dtype,
                                    void* workspace, size_t workspace_bytes, void* stream) {
   if (!k_cache || !v_cache || !cu_seqlens || !seq_lens) return DBK_ENULL;
+  const bool two = !(dtype & DBK_WEIGHTS_ONE);
+  dtype &= ~DBK_WEIGHTS_ONE;
   if (dtype != DBK_F16 && dtype != DBK_BF16) return DBK_EDTYPE;
   if (head_dim != kHd || tokens < 0 || batch < 1 || n_kv_heads < 1 || n_q_heads < n_kv_heads ||
       n_q_heads % n_kv_heads != 0 || num_pages < 1 || page_size < 1)
@@ -1178,5 +1237,6 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   rc = encode_tmap_2d(&a.vmap, v_cache, dtype, kHd, cache_rows, kHd * 2, 64, box, true);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == DBK_F16 ? launch<__half>(a, dev, st) : launch<__nv_bfloat16>(a, dev, st);
+  if (dtype == DBK_F16) return two ? launch<__half, true>(a, dev, st) : launch<__half, false>(a, dev, st);
+  return two ? launch<__nv_bfloat16, true>(a, dev, st) : launch<__nv_bfloat16, false>(a, dev, st);
 }

@@ -31,6 +31,7 @@ extern "C" {
 /* Element type of activations, weights, caches and outputs. */
 typedef enum { DBK_F16 = 0, DBK_BF16 = 1 } dbk_dtype;
 #define DBK_F32 2             /* logits of dbk_sample only */
+#define DBK_WEIGHTS_ONE 0x100 /* added to the dtype of dbk_chunk_attention, see there */
 
 /* Argument errors (negative). Positive values are cudaError_t. */
 #define DBK_OK 0
@@ -299,7 +300,10 @@ int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* sl
  *   q head h reads kv head h / (n_q_heads / n_kv_heads), any ratio up to 128. scale > 0.
  * Rows of out behind cu_seqlens[batch] are left as they were. Cache slots at and past seq_lens
  * may hold anything, and values that are not finite reach only the rows that see them. Maximum,
- * sum and output accumulate in fp32; the weights are rounded to dtype for the tensor cores. out
+ * sum and output accumulate in fp32. The tensor cores get a weight as the sum of two values of
+ * dtype, so the result's own rounding is the only one of its size; with dtype | DBK_WEIGHTS_ONE
+ * as one value, which is faster and adds half a step of dtype of the weighted |v|. (fp16: no step of a
+ * weight is smaller than 2^-36 of the row's largest.) out
  * does not overlap q; batch <= 65536. Results do not depend on timing.
  * workspace: dbk_chunk_attention_workspace_bytes(), need not be zero-filled, one per call that
  * may run concurrently. */
