@@ -33,9 +33,9 @@
 //
 // Rounding. The answer is an index, and a cut that falls on another side of a sum changes it,
 // so weights and sums are wider than 32-bit floats: common path, 30-bit weights (Exp2Table) as
-// 64-bit integers, whose order of addition does not matter; general path, weights above 2^-kFine
-// of the largest by 64-bit exp(), smaller ones by 32-bit exponentials (2^-21 of at most
-// 2^-kFine), sums in doubles in a fixed order.
+// 64-bit integers, whose order of addition does not matter; general path, weights by 64-bit exp()
+// (2^-46 of each: its argument is rounded too), summed in doubles in a fixed order, or for a cut as
+// integers of 2^-61 of the row's sum and less.
 #include <climits>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -54,8 +54,8 @@ namespace {
 // row of 128,000: 24 us with 512 threads; two to an SM, with 64 registers: 27).
 constexpr int kManyThreads = 256, kManyCtas = 3, kFewThreads = 512, kMaxWarps = 32;
 constexpr int kBins = 256;
-constexpr float kFine = 14.f;       // log2 distance up to which weights are 64-bit
-constexpr float kFar = 46.f;        // and past which they are nothing
+constexpr float kFine = 14.f;       // log2 distances of the general path's first histogram
+constexpr float kFar = 46.f;        // and of its second; past it weights are nothing to the common path
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxSlice = 32768;    // logits of a CTA, at most (with 256 threads 32 rounds of a warp)
@@ -84,7 +84,7 @@ struct Hist {
 struct SampleShared {
   Hist hist[2];                       // alternate between passes: one cluster barrier each
   double sum[2];
-  unsigned long long idx[2];
+  unsigned long long far[2], idx[2];
   float top[2];
   double warp_d[kMaxWarps];
   unsigned long long warp_m[kMaxWarps];
@@ -228,11 +228,12 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
   int phase = 0;
   const float cl = log2_per_logit(temp);
   const double dM = (double)M, dT = (double)temp;
-  auto dist = [&](float x) { return (x == M ? 0.f : M - x) * cl; };          // log2 of max w / w
-  auto fine = [&](float x) { return x == M ? 1.0 : exp(((double)x - dM) / dT); };
-  auto fixed = [&](float x, float d) -> unsigned long long {
-    const double w = d < kFine ? fine(x) : (double)fast_ex2(-d);
-    return (unsigned long long)__double2ll_rn(w * a.unit);
+  auto dist = [&](float x) { return (x == M ? 0.f : M - x) * cl; };          // log2 of max w / w, for bins
+  auto fine = [&](float x) -> double {                                       // w
+    if (x == M) return 1.0;
+    if (x == -INFINITY) return 0.0;
+    const double w = exp(((double)x - dM) / dT);
+    return w > 0.0 ? w : 0.0;                       // (0 / 0 of infinite logits and temperatures)
   };
 
   // Find the first index, in index order, at which the running sum of value(x, i) over the whole
@@ -359,39 +360,65 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
   if (by_k || by_p) {
     // One pass: `place` gives a logit's bin (or -1), the histograms of all CTAs are joined, and
     // cum_count / cum_mass hold their running sums.
-    double rest = 0.0;                              // mass of the logits `place` sends past the end
+    // Units of a weight: the row's sum takes 61 to 62 bits of 63, whatever its logits are, so that a
+    // rounding of each of 2^20 weights is 2^-42 of it.
+    double unit = 1.0;
+    auto fixed = [&](float x) { return by_p ? (unsigned long long)__double2ll_rn(fine(x) * unit) : 0ull; };
+    if (by_p) {
+      double z = 0.0;
+      for (int v = v0 + tid; v < v1; v += NT) {
+        float f[VN];
+        load(v, f);
+        float some = 0.f;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) some += fast_ex2(-dist(f[e]));
+        z += (double)some;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (lane == 0) sh.warp_d[warp] = z;
+      __syncthreads();
+      const int ph = phase++ & 1;
+      if (tid == 0) {
+        double t = 0.0;
+        for (int w = 0; w < (NT / 32); ++w) t += sh.warp_d[w];
+        sh.sum[ph] = t;
+      }
+      cluster.sync();
+      z = 0.0;
+      for (int r = 0; r < C; ++r) z += *cluster.map_shared_rank(&sh.sum[ph], r);
+      unit = ldexp(1.0, 61 - ilogb(fmax(z, 1.0)));  // (z is right to 2^-10)
+    }
+    unsigned long long rest = 0;                    // mass of the logits `place` sends past the end
     auto histogram = [&](auto&& place, bool first) {
       const int ph = phase++ & 1;
       Hist& h = sh.hist[ph];
       for (int i = tid; i < kBins; i += NT) { h.mass[i] = 0; h.count[i] = 0; }
       __syncthreads();
-      double tail = 0.0;
+      unsigned long long tail = 0;
       for (int v = v0 + tid; v < v1; v += NT) {
         float f[VN];
         load(v, f);
-        float far = 0.f;
 #pragma unroll
         for (int e = 0; e < VN; ++e) {
-          const float d = dist(f[e]);
-          const int b = place(f[e], d);
+          const int b = place(f[e], dist(f[e]));
           if (b >= 0) {
             atomicAdd(&h.count[b], 1u);
-            atomicAdd(&h.mass[b], fixed(f[e], d));
+            if (by_p) atomicAdd(&h.mass[b], fixed(f[e]));
           } else if (first) {
-            far += fast_ex2(-d);
+            tail += fixed(f[e]);
           }
         }
-        tail += (double)far;
       }
       if (first) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) tail += __shfl_xor_sync(0xffffffffu, tail, o);
-        if (lane == 0) sh.warp_d[warp] = tail;
+        if (lane == 0) sh.warp_m[warp] = tail;
         __syncthreads();
         if (tid == 0) {
-          double t = 0.0;
-          for (int w = 0; w < (NT / 32); ++w) t += sh.warp_d[w];
-          sh.sum[ph] = t;
+          unsigned long long t = 0;
+          for (int w = 0; w < (NT / 32); ++w) t += sh.warp_m[w];
+          sh.far[ph] = t;
         }
       }
       cluster.sync();
@@ -405,8 +432,8 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
         }
       }
       if (first) {
-        rest = 0.0;
-        for (int r = 0; r < C; ++r) rest += *cluster.map_shared_rank(&sh.sum[ph], r);
+        rest = 0;
+        for (int r = 0; r < C; ++r) rest += *cluster.map_shared_rank(&sh.far[ph], r);
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -443,45 +470,48 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
     auto wide_bin = [&](float, float d) {
       return d >= kFine && d < kFar ? min((int)((d - kFine) * kWide), kBins - 1) : -1;
     };
+    auto past_bin = [&](float x, float d) { return d >= kFar && x > -INFINITY ? 0 : -1; };
 
     // The prefix that reaches `need` (a count, or a mass): sets kx and cut; returns its mass.
     // The first histogram has been made already.
     auto search = [&](bool count, unsigned long long need) -> unsigned long long {
       unsigned long long above = 0;                 // mass above the current range
-      int b = crossing(count, need);
-      bool wide = false;
-      if (b == kBins) {                             // past the first histogram: the far one
-        const unsigned long long got = count ? (unsigned long long)sh.cum_count[kBins - 1] : sh.cum_mass[kBins - 1];
-        above = sh.cum_mass[kBins - 1];
-        need -= got;
+      int b = crossing(count, need), stage = 0;
+      auto take = [&](int n) {                      // the first n bins lie in front
+        if (n == 0) return;
+        need -= count ? (unsigned long long)sh.cum_count[n - 1] : sh.cum_mass[n - 1];
+        above += sh.cum_mass[n - 1];
         __syncthreads();
-        histogram(wide_bin, false);
+      };
+      while (b == kBins) {                          // past this histogram: the next
+        take(kBins);
+        if (++stage == 3) { kx = 0; cut = -1; return above; }      // all that weigh anything
+        if (stage == 1) histogram(wide_bin, false);
+        else histogram(past_bin, false);
         b = crossing(count, need);
-        wide = true;
-        if (b == kBins) { kx = 0; cut = -1; return above + sh.cum_mass[kBins - 1]; }   // everything
       }
-      if (b > 0) { need -= count ? (unsigned long long)sh.cum_count[b - 1] : sh.cum_mass[b - 1]; above += sh.cum_mass[b - 1]; }
-      __syncthreads();
+      take(b);
       // Keys the bin can hold: its edges, four values more on each side (the distance has three
       // roundings), members by the bin itself.
-      const float lo = wide ? kFine + b / kWide : b / kNear, hi = wide ? kFine + (b + 1) / kWide : (b + 1) / kNear;
+      const float lo = stage == 2 ? kFar : stage == 1 ? kFine + b / kWide : b / kNear;
+      const float hi = stage == 2 ? INFINITY : stage == 1 ? kFine + (b + 1) / kWide : (b + 1) / kNear;
       unsigned int khi = order_key(M - lo / cl * (1.f - 2e-6f)), klo = order_key(M - hi / cl * (1.f + 2e-6f));
       khi = khi > 0xffffffffu - 4 ? 0xffffffffu : khi + 4;
-      klo = klo < 5 ? 1 : klo - 4;
+      klo = stage == 2 || klo < 5 ? 1 : klo - 4;
       // from here up a key is surely not of a later bin
-      const unsigned int sure = order_key(M - hi / cl * (1.f - 2e-6f)) + 4;
+      const unsigned int sure = stage == 2 ? 0 : order_key(M - hi / cl * (1.f - 2e-6f)) + 4;
       const int bin = b;
       for (;;) {
         int shift = 0;
         while (((khi - klo) >> shift) >= kBins) ++shift;
         histogram([&](float x, float d) {
-          if ((wide ? wide_bin(x, d) : near_bin(x, d)) != bin) return -1;
+          if ((stage == 2 ? past_bin(x, d) : stage == 1 ? wide_bin(x, d) : near_bin(x, d)) != bin) return -1;
           const unsigned int key = order_key(x);
           return key > khi || key < klo ? -1 : (int)((khi - key) >> shift);
         }, false);
         b = crossing(count, need);
         if (b == kBins) b = kBins - 1;              // cannot be: the bin's members are in the range
-        if (b > 0) { need -= count ? (unsigned long long)sh.cum_count[b - 1] : sh.cum_mass[b - 1]; above += sh.cum_mass[b - 1]; }
+        take(b);
         const unsigned int n = sh.cum_count[b] - (b > 0 ? sh.cum_count[b - 1] : 0);
         const unsigned long long m = sh.cum_mass[b] - (b > 0 ? sh.cum_mass[b - 1] : 0);
         __syncthreads();
@@ -489,27 +519,27 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
         const unsigned int width = 1u << shift;
         if (khi - klo >= width) klo = khi - width + 1;
         if ((n <= 1 && klo >= sure) || klo == khi) {
-          // One logit, or n equal ones of which the first `take` by index are kept.
-          unsigned long long take = n;
-          if (n > 1) take = count ? need : (m / n == 0 ? n : (need + m / n - 1) / (m / n));
-          if (take >= n) {
+          // One logit, or n equal ones of which the first `kept` by index stay.
+          unsigned long long kept = n;
+          if (n > 1) kept = count ? need : (m / n == 0 ? n : (need + m / n - 1) / (m / n));
+          if (kept >= n) {
             kx = klo - 1;
             cut = -1;
             return above + m;
           }
           kx = klo;
           auto tie = [&](float x, int) { return order_key(x) == kx ? 1.0 : 0.0; };
-          const double last = (double)take - 1.0;
+          const double last = (double)kept - 1.0;
           // (with the histogram still wanted by the caller this is only reached last)
           cut = locate(sum_of(tie), tie, [&](double) { return last; });
-          return above + m / n * take;
+          return above + m / n * kept;
         }
       }
     };
 
     histogram(near_bin, true);
     const unsigned long long near_mass = sh.cum_mass[kBins - 1];
-    unsigned long long Z = near_mass + (unsigned long long)__double2ll_rn(rest * a.unit);
+    unsigned long long Z = near_mass + rest;
     bool fresh = true;                              // the first histogram is in cum_*
     if (by_k) {
       Z = search(true, (unsigned long long)k);
@@ -525,24 +555,20 @@ __device__ __noinline__ void general_row(const SampleArgs& a, const Row& R, floa
   // ---------------------------------------------------------------- the draw
   const bool cuts = by_k || by_p;
   const bool low = mp > 0.f;
-  auto kept = [&](float x, int i, float d) {
-    if (d >= kFar) return false;
+  auto kept = [&](float x, int i) {
     if (cuts) {
       const unsigned int key = order_key(x);
       if (!(key > kx || (key == kx && i <= cut))) return false;
     }
-    if (low) {
-      const float w = fast_ex2(-d);
-      if (w < mp * 0.999f) return false;
-      if (w <= mp * 1.001f) return fine(x) >= (double)mp;
+    if (low) {                                      // by the 32-bit weight but next to the border
+      const float d = dist(x), w = fast_ex2(-d);
+      if (w > mp * 1.001f) return true;
+      if (w < mp * 0.999f && (mp > 1e-30f || d < 100.f)) return false;
+      return fine(x) >= (double)mp;
     }
     return true;
   };
-  auto weight = [&](float x, int i) {
-    const float d = dist(x);
-    if (!kept(x, i, d)) return 0.0;
-    return d < kFine ? fine(x) : (double)fast_ex2(-d);
-  };
+  auto weight = [&](float x, int i) { return kept(x, i) ? fine(x) : 0.0; };
   const int i = locate(sum_of(weight), weight, [&](double total) { return (double)R.u * total; });
   if (rank == 0 && tid == 0) a.out[row] = i;
   cluster.sync();
