@@ -859,7 +859,9 @@ __global__ void __launch_bounds__(NT, NT == kManyThreads ? kManyCtas : 1) sample
   const double dM = (double)M;
   const double per = fmax(fmin(1.4426950408889634 / fmax((double)R.temp, 1e-38), 1e30), 1e-30);
   const float places = cl * (8.f * kBinsPerLog2);
-  auto place = [&](float v) { return (M - v) * places; };      // distance in eighths of a bin
+  // Distance in eighths of a bin. Every pass forms it anew and must get the same value: rounded here,
+  // so that no pass's product goes unrounded into a sum of its own.
+  auto place = [&](float v) { return __fmul_rn(__fsub_rn(M, v), places); };
   auto units = [&](float v) { return sh.table((double)v - dM, per, a.lower_bits); };   // place < kPlaces
   // w >= min_p: by the units but for those next to the border.
   const double mp_units = (double)R.mp * a.unit;

@@ -128,3 +128,31 @@ def test_infinite_logits_and_a_cut_behind_them():
     got = ops.sample(x.cuda()[None].expand(5, -1).contiguous(), torch.tensor([0.0, 0.4, 0.9, 0.5, 0.999]).cuda(),
                      top_k=torch.tensor([0, 3, 2, 1, 1000], dtype=torch.int32, device="cuda"))
     assert got.tolist() == [5, 77, 77, 5, 299999]
+
+
+def test_a_logit_that_rounds_onto_a_bin_border():
+    """Distances whose product with the bins per logit lies just below the border of two bins and rounds
+    onto it: every pass has to put the logit into the same bin. The cut falls into the second of
+    the two, behind more logits than the lists hold; the last kept one has the highest index."""
+    vocab, front = 32003, 6000
+    scale = np.float32(np.float32(1.4426950408889634) * np.float32(8 * np.float32(np.float32(512) / np.float32(46))))
+    rows, last = [], []
+    for b in range(2, 40):
+        edge = 8 * b - 0.5
+        d = np.float32(edge / float(scale))
+        near = [d, np.nextafter(d, np.float32(0)), np.nextafter(d, np.float32(9))]
+        hit = [v for v in near if np.float32(v * scale) == np.float32(edge) and float(v) * float(scale) < edge]
+        if not hit:
+            continue
+        x = torch.full((vocab,), -31.0)
+        x[0] = 0.0
+        x[1:1 + front] = -(8 * (b - 1) + 3) / float(scale)
+        x[front + 50] = -float(hit[0])
+        x[20000:20300] = -(8 * b + 0.2 + torch.arange(300) * 0.02) / float(scale)
+        rows.append(x)
+        last.append(20000 + 149)
+    assert len(rows) > 10
+    x, u = torch.stack(rows[:8]).cuda(), torch.full((8,), 1 - 2.0 ** -24, device="cuda")
+    assert ops.sample(x, u, top_k=front + 2 + 150).tolist() == last[:8]
+    x, u = torch.stack(rows[8:]).cuda(), torch.full((len(rows) - 8,), 1 - 2.0 ** -24, device="cuda")
+    assert ops.sample(x, u, top_k=front + 2 + 150).tolist() == last[8:]
