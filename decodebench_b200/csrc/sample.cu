@@ -33,9 +33,10 @@
 //
 // Rounding. The answer is an index, and a cut that falls on another side of a sum changes it,
 // so weights and sums are wider than 32-bit floats: common path, 30-bit weights (Exp2Table) as
-// 64-bit integers, whose order of addition does not matter; general path, weights by 64-bit exp()
-// (2^-46 of each: its argument is rounded too), summed in doubles in a fixed order, or for a cut as
-// integers of 2^-61 of the row's sum and less.
+// 64-bit integers, whose order of addition does not matter, cut off to units of 2^-45 of the largest (2^-43
+// for 2^18 logits) and dropped below 2^-46 of it: a sum is right to 2^-28 of itself and a unit for
+// each logit. General path, weights by 64-bit exp() (2^-46 of each: its argument is rounded too),
+// summed in doubles in a fixed order, or for a cut as integers of 2^-61 of the row's sum and less.
 #include <climits>
 #include <cmath>
 #include <cooperative_groups.h>
@@ -829,7 +830,9 @@ __global__ void __launch_bounds__(NT, NT == kManyThreads ? kManyCtas : 1) sample
     cluster.sync();
     return;
   }
-  if (M == INFINITY && !greedy) {                  // infinite logits share the draw
+  // To the general path: infinite logits, which share the draw; draws that may end among the weights this path
+  // drops (2^18 of less than 2^-46: 2^-28 of the largest).
+  if ((M == INFINITY || R.u < 0x1p-24f) && !greedy) {
     cluster.sync();
     general_row<T, NT>(a, R, M, *reinterpret_cast<SampleShared*>(dyn), dyn + sizeof(SampleShared) / sizeof(double));
     return;

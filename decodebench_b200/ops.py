@@ -708,7 +708,9 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=
     token is the first index whose running sum of kept weights exceeds uniforms[b] (fp32, in
     [0, 1)) times their sum; temperature <= 0 takes the largest logit. Each parameter is a
     number or a tensor [batch] (fp32, ``top_k`` int32; None, top_k <= 0, top_p >= 1 and
-    min_p <= 0 are off). NaN counts as -inf; a row of nothing but -inf gives -1."""
+    min_p <= 0 are off). NaN counts as -inf; a row of nothing but -inf gives -1. Sums are wider
+    than 32-bit floats but not exact: ``dbk_sample`` says how near a border a draw may fall on
+    its other side. ``logits`` must be contiguous and start on 16 bytes."""
     dev = _cuda_device(logits, uniforms, *[t for t in (temperature, top_k, top_p, min_p)
                                            if isinstance(t, torch.Tensor)])
     if logits.dim() != 2:

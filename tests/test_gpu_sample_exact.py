@@ -93,7 +93,7 @@ def test_tails_of_16_bit_logits(dt):
 def test_crowded_rows_of_a_common_vocabulary():
     """Rows that overflow the common path's lists: many equal logits at the cut, far below the largest."""
     x, u = tail(120000, "flat", 5)
-    check_rows(x, u, GENERAL, top_p=0.9)
+    check_rows(x, u, GENERAL, top_p=0.97)
     check_rows(x, u, GENERAL, temperature=0.8, top_k=70000)
 
 
@@ -156,3 +156,19 @@ def test_a_logit_that_rounds_onto_a_bin_border():
     assert ops.sample(x, u, top_k=front + 2 + 150).tolist() == last[:8]
     x, u = torch.stack(rows[8:]).cuda(), torch.full((len(rows) - 8,), 1 - 2.0 ** -24, device="cuda")
     assert ops.sample(x, u, top_k=front + 2 + 150).tolist() == last[8:]
+
+
+@pytest.mark.parametrize("dt,vocab", [(F32, 9), (F16, 1000), (BF16, 32003), (F32, 128000)])
+def test_draws_among_the_smallest_weights(dt, vocab):
+    """Draws of 0, and below the step of 24-bit random numbers, in rows of the common path: the first
+    index that is kept and weighs anything, however little."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(vocab, generator=g)
+    x[0], x[1], x[2] = -math.inf, -900.0, -60.0
+    x = x.to(dt)
+    u = torch.tensor([0.0, 1e-44, 1e-30, 2.0 ** -40, 2.0 ** -25, 2.0 ** -24, 2.0 ** -20])
+    check_rows(x, u[:6], GENERAL)
+    assert ops.sample(x.cuda()[None], u[:1].cuda()).tolist() == [2]
+    check_rows(x, u, 2.0 ** -25, temperature=0.5)
+    for f in (dict(top_k=vocab - 2), dict(top_k=5), dict(top_p=0.99), dict(top_k=40, top_p=0.9)):
+        check_rows(x, u, 2.0 ** -25, **f)
