@@ -156,7 +156,8 @@ __device__ __forceinline__ Row load_row(const SampleArgs& a) {
   r.temp = a.temperature ? __ldcg(a.temperature + r.row) : a.temp;
   r.k = a.top_k ? __ldcg(a.top_k + r.row) : a.k;
   r.p = a.top_p ? __ldcg(a.top_p + r.row) : a.p;
-  r.mp = fminf(a.min_p ? __ldcg(a.min_p + r.row) : a.mp, 1.f);
+  r.mp = a.min_p ? __ldcg(a.min_p + r.row) : a.mp;
+  r.mp = r.mp > 0.f ? fminf(r.mp, 1.f) : 0.f;             // (NaN: off)
   r.u = fminf(fmaxf(__ldcg(a.u + r.row), 0.f), 0x1.fffffep-1f);
   // The row in whole 16-byte vectors: vector 0 starts `head` logits before it.
   const long long start = (long long)r.row * a.vocab;

@@ -323,8 +323,9 @@ size_t dbk_chunk_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_
  *   tokens[b] (int64) = the first index whose running sum of kept weights, in index order,
  *   exceeds uniforms[b] * their sum. temperature <= 0: the first of the order.
  * temperature, top_k, top_p, min_p: device arrays [batch], or NULL for the value given for all
- * rows (top_k <= 0, top_p >= 1, min_p <= 0: off). NaN logits count as -inf; a row with
- * nothing but -inf gives -1; logits of +inf share the draw alike. min_p above 1 keeps what
+ * rows (top_k <= 0, top_p >= 1, min_p <= 0: off; NaN in an array: temperature 0, the others off).
+ * NaN logits count as -inf; a row with nothing but -inf gives -1; logits of +inf share the draw
+ * alike. min_p above 1 keeps what
  * min_p = 1 keeps. Weights (that of exp() in 64 bits, 0 where it is 0) and sums do not depend on
  * timing. A row with more than 2^18 logits, with many near or equal ones at a cut, or with
  * uniforms[b] < 2^-24 is decided to 2^-41 of its sum; others have weights of 30 bits in units of

@@ -172,3 +172,16 @@ def test_draws_among_the_smallest_weights(dt, vocab):
     check_rows(x, u, 2.0 ** -25, temperature=0.5)
     for f in (dict(top_k=vocab - 2), dict(top_k=5), dict(top_p=0.99), dict(top_k=40, top_p=0.9)):
         check_rows(x, u, 2.0 ** -25, **f)
+
+
+def test_parameters_that_are_not_numbers():
+    """NaN among the rows' parameters: top-p and min-p are off, temperature takes the largest logit."""
+    x = torch.randn(4, 5000, generator=torch.Generator().manual_seed(1)).cuda()
+    u = torch.tensor([0.3, 0.7, 0.9, 0.5]).cuda()
+    nan = torch.full((4,), math.nan, device="cuda")
+    plain = ops.sample(x, u)
+    assert torch.equal(ops.sample(x, u, min_p=nan), plain)
+    assert torch.equal(ops.sample(x, u, top_p=nan), plain)
+    assert torch.equal(ops.sample(x, u, temperature=nan), x.argmax(1))
+    big = torch.randn(2, 300001, generator=torch.Generator().manual_seed(2)).cuda()
+    assert torch.equal(ops.sample(big, u[:2], min_p=nan[:2]), ops.sample(big, u[:2]))
