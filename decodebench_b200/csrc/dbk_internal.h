@@ -41,6 +41,27 @@ inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y ? y - x < a_bytes : x - y < b_bytes;
 }
+struct Span {
+  const void* p;     // NULL or no bytes: not there
+  size_t bytes;
+};
+// Some output overlaps an input or another output.
+template <int NO, int NI>
+inline bool outputs_overlap(const Span (&outs)[NO], const Span (&ins)[NI]) {
+  auto meet = [](const Span& a, const Span& b) { return a.p && b.p && a.bytes && b.bytes && overlap(a.p, a.bytes, b.p, b.bytes); };
+  for (int i = 0; i < NO; ++i) {
+    for (int j = i + 1; j < NO; ++j)
+      if (meet(outs[i], outs[j])) return true;
+    for (const Span& in : ins)
+      if (meet(outs[i], in)) return true;
+  }
+  return false;
+}
+// Bytes of a cache of rows of 128 16-bit values; all there are where the product does not fit.
+inline size_t cache_bytes(int64_t pages, int64_t heads, int64_t page_size) {
+  const double b = 256.0 * (double)pages * (double)heads * (double)page_size;
+  return b < 9e18 ? (size_t)pages * heads * page_size * 256 : SIZE_MAX;
+}
 
 // Encode a 2-D tiled TMA descriptor over a row-major [rows, inner] matrix of
 // 16-bit elements (dtype DBK_F16 / DBK_BF16), box [box_rows, box_inner], with

@@ -276,8 +276,11 @@ extern "C" int dbk_rope_append(const void* qkv, const int32_t* positions, const 
   if (!qkv || !positions || !slots || !q_out) return DBK_ENULL;
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache))
     return DBK_EALIGN;
-  if (overlap(qkv, (size_t)tokens * (n_q_heads + 2 * n_kv_heads) * 256, q_out, (size_t)tokens * n_q_heads * 256))
-    return DBK_ESHAPE;
+  const size_t cache = cache_bytes(num_pages, n_kv_heads, page_size);
+  const Span outs[] = {{q_out, (size_t)tokens * n_q_heads * 256}, {k_cache, cache}, {v_cache, cache}};
+  const Span ins[] = {{qkv, (size_t)tokens * (n_q_heads + 2 * n_kv_heads) * 256}, {positions, (size_t)tokens * 4},
+                      {slots, (size_t)tokens * 8}, {inv_freq, 256}};
+  if (outputs_overlap(outs, ins)) return DBK_ESHAPE;
   DeviceInfo dev;
   if (int rc = current_device_info(&dev)) return rc;
   RopeArgs a{};

@@ -281,8 +281,9 @@ int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_
  *   inv_freq[i], formed in 64 bits); q -> q_out [tokens, n_q_heads, 128]; k, v -> slot slots[t] of
  *   k_cache, v_cache [num_pages, n_kv_heads, page_size, 128] (a contiguous cache [batch,
  *   n_kv_heads, max_len, 128] is one page per sequence: slot = b * max_len + position).
- * q_out does not overlap qkv. A slot outside the cache (-1 for a padded row) writes q only. Slots must differ from one
- * another; of two rows with one slot either may be kept, in parts. head_dim 128 only. */
+ * q_out and the caches overlap neither one another nor an input (DBK_ESHAPE). A slot outside the
+ * cache (-1 for a padded row) writes q only. Slots must differ from one another; of two rows with
+ * one slot either may be kept, in parts. head_dim 128 only. */
 int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* slots,
                     const float* inv_freq, void* q_out, void* k_cache, void* v_cache, int tokens,
                     int n_q_heads, int n_kv_heads, int head_dim, int num_pages, int page_size,

@@ -5,7 +5,7 @@ import pytest
 pytest.importorskip("torch")
 
 from decodebench_b200 import _native as N  # noqa: E402
-from tests.test_paged_cpu import EDTYPE, ENULL, attend  # noqa: E402
+from tests.test_paged_cpu import EDTYPE, ENULL, ESHAPE, append, attend  # noqa: E402
 
 
 @pytest.mark.parametrize("dt,want", [
@@ -13,3 +13,16 @@ from tests.test_paged_cpu import EDTYPE, ENULL, attend  # noqa: E402
     (N.DBK_F16 | N.DBK_WEIGHTS_ONE, ENULL)])
 def test_chunk_attention_weight_parts(dt, want):
     assert attend(dt=dt, q=None) == want
+
+
+# Addresses that nothing is read from: every call here is refused. 3 tokens, 4 / 2 heads, 4 pages of 16:
+# q 3,072 bytes, qkv 6,144, a cache 32,768.
+APART = dict(qkv=0x100000, q=0x200000, k=0x300000, v=0x400000, pos=0x500000, slots=0x600000, inv=0x700000)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=0x300000 + 32768 - 16), dict(q=0x300000 - 3072 + 16), dict(q=0x400000), dict(k=0x400000 + 16),
+    dict(v=0x300000), dict(qkv=0x300000 + 16), dict(qkv=0x400000 - 6144 + 16), dict(qkv=0x200000 + 3072 - 16),
+    dict(pos=0x200000), dict(slots=0x300000 + 64), dict(inv=0x400000 + 32768 - 4)])
+def test_rope_append_outputs_that_overlap(kw):
+    assert append(**{**APART, **kw}) == ESHAPE
