@@ -1197,7 +1197,11 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   if (!q || !out) return DBK_ENULL;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return DBK_EALIGN;
   const size_t q_bytes = (size_t)tokens * n_q_heads * kHd * 2;
-  if (overlap(q, q_bytes, out, q_bytes)) return DBK_ESHAPE;
+  const size_t cache = cache_bytes(num_pages, n_kv_heads, page_size);
+  const Span outs[] = {{out, q_bytes}, {workspace, workspace_bytes}};
+  const Span ins[] = {{q, q_bytes}, {k_cache, cache}, {v_cache, cache}, {cu_seqlens, ((size_t)batch + 1) * 4},
+                      {seq_lens, (size_t)batch * 4}, {page_table, page_table ? (size_t)batch * max_pages_per_seq * 4 : 0}};
+  if (outputs_overlap(outs, ins)) return DBK_ESHAPE;
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;

@@ -631,7 +631,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with p < 0 gives zeros. Chunks of any length, of 0 and of 1 token included. Paged caches
     (``page_table`` int32 [batch, max_pages]): k/v [pages, Hkv, page_size, 128], page_size a
     multiple of 8; contiguous: [batch, Hkv, max_len, 128]. ``scale`` (> 0) defaults to
-    1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` (which must not overlap q) are left as
+    1/sqrt(128). Rows behind cu_seqlens[batch] of ``out`` (which overlaps no input) are left as
     they were.
 
     ``weight_parts``: the tensor cores get each softmax weight as the sum of two values of the

@@ -304,8 +304,9 @@ int dbk_rope_append(const void* qkv, const int32_t* positions, const int64_t* sl
  * sum and output accumulate in fp32. The tensor cores get a weight as the sum of two values of
  * dtype, so the result's own rounding is the only one of its size; with dtype | DBK_WEIGHTS_ONE
  * as one value, which is faster and adds half a step of dtype of the weighted |v|. (fp16: no step of a
- * weight is smaller than 2^-36 of the row's largest.) out
- * does not overlap q; batch <= 65536. Results do not depend on timing.
+ * weight is smaller than 2^-36 of the row's largest.) out and the workspace overlap neither each
+ * other nor an input (DBK_ESHAPE); k_cache and v_cache may be one. batch <= 65536. Results do not
+ * depend on timing.
  * workspace: dbk_chunk_attention_workspace_bytes(), need not be zero-filled, one per call that
  * may run concurrently. */
 int dbk_chunk_attention(const void* q, const void* k_cache, const void* v_cache,

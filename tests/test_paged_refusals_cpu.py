@@ -26,3 +26,20 @@ APART = dict(qkv=0x100000, q=0x200000, k=0x300000, v=0x400000, pos=0x500000, slo
     dict(pos=0x200000), dict(slots=0x300000 + 64), dict(inv=0x400000 + 32768 - 4)])
 def test_rope_append_outputs_that_overlap(kw):
     assert append(**{**APART, **kw}) == ESHAPE
+
+
+def attend_apart(ws=0x500000, ws_bytes=1 << 16, **kw):
+    a = dict(q=0x100000, out=0x200000, k=0x300000, v=0x400000, cu=0x600000, lens=0x610000, table=0x620000,
+             n=3, batch=2, hq=4, hkv=2, d=128, pages=4, page=16, width=8, scale=0.1, dt=0)
+    a.update(kw)
+    return N.load().dbk_chunk_attention(*[a[k] for k in (
+        "q", "k", "v", "cu", "lens", "table", "out", "n", "batch", "hq", "hkv", "d", "pages", "page",
+        "width", "scale", "dt")], ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=0x300000), dict(out=0x300000 + 32768 - 16), dict(out=0x400000 - 16), dict(cu=0x200000 + 3068),
+    dict(lens=0x200000), dict(table=0x200000 - 60), dict(ws=0x200000 + 3072 - 16), dict(ws=0x400000 - (1 << 16) + 16),
+    dict(ws=0x100000), dict(ws=0x610000 - 256, ws_bytes=512)])
+def test_chunk_attention_outputs_that_overlap(kw):
+    assert attend_apart(**kw) == ESHAPE
