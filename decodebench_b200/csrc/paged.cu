@@ -246,6 +246,11 @@ extern "C" int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens,
       tokens < 0 || (int64_t)batch * max_pages_per_seq > INT_MAX)
     return DBK_ESHAPE;
   if ((n_free > 0 && !free_pages) || (tokens > 0 && (!positions || !slots))) return DBK_ENULL;
+  const size_t lens = (size_t)batch * 4;
+  const Span outs[] = {{page_table, lens * max_pages_per_seq}, {seq_lens, lens}, {cu_seqlens, lens + 4},
+                       {positions, (size_t)tokens * 4}, {slots, (size_t)tokens * 8}, {used, 4}};
+  const Span ins[] = {{ctx_lens, lens}, {new_lens, lens}, {free_pages, (size_t)n_free * 4}};
+  if (outputs_overlap(outs, ins)) return DBK_ESHAPE;
   DeviceInfo dev;
   if (int rc = current_device_info(&dev)) return rc;
   PlanArgs a{};

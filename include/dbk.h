@@ -268,8 +268,8 @@ int dbk_gateup_swiglu_fp8(const void* x, const void* gamma, const void* Wg8, con
  *                       is no page (list or table too short). Rows behind the last
  *                       token get position 0 and slot -1; tokens behind the `tokens`-th are left out.
  *   used                int32 [1]: free pages the step needs (more than n_free: it lacked some)
- * Requests' token total and lengths stay below 2^31; batch <= 16384; outputs must not overlap
- * inputs. Any later call may follow directly: the plan is complete before it starts. */
+ * Requests' token total and lengths stay below 2^31; batch <= 16384; outputs overlap neither
+ * inputs nor one another (DBK_ESHAPE). Any later call may follow directly: the plan is complete before it starts. */
 int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_pages,
                   int32_t* page_table, int32_t* seq_lens, int32_t* cu_seqlens,
                   int32_t* positions, int64_t* slots, int32_t* used, int batch, int n_free,
