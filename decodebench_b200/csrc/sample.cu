@@ -1327,6 +1327,11 @@ extern "C" int dbk_sample(const void* logits, const float* uniforms, const float
   if (batch == 0) return DBK_OK;
   if (!logits || !uniforms || !tokens) return DBK_ENULL;
   if (!aligned16(logits)) return DBK_EALIGN;
+  const size_t rows = (size_t)batch * 4;
+  const Span outs[] = {{tokens, 2 * rows}};
+  const Span ins[] = {{logits, (size_t)batch * vocab * (dtype == DBK_F32 ? 4 : 2)}, {uniforms, rows},
+                      {temperature, rows}, {top_k, rows}, {top_p, rows}, {min_p, rows}};
+  if (outputs_overlap(outs, ins)) return DBK_ESHAPE;
   DeviceInfo dev;
   if (int rc = current_device_info(&dev)) return rc;
   SampleArgs a{};

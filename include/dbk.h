@@ -332,7 +332,8 @@ size_t dbk_chunk_attention_workspace_bytes(int64_t tokens, int n_q_heads, int n_
  * timing. A row with more than 2^18 logits, with many near or equal ones at a cut, or with
  * uniforms[b] < 2^-24 is decided to 2^-41 of its sum; others have weights of 30 bits in units of
  * 2^-45 of the largest (2^-43 for 2^18 logits), cut off, which decides to 2^-28 of the sum and a
- * unit for each logit. uniforms[b] = 0 takes the first index that is kept and weighs anything. */
+ * unit for each logit. uniforms[b] = 0 takes the first index that is kept and weighs anything.
+ * tokens overlaps no input (DBK_ESHAPE). */
 int dbk_sample(const void* logits, const float* uniforms, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens,
                int batch, int vocab, float temperature_all, int top_k_all, float top_p_all,

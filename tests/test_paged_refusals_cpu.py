@@ -5,7 +5,7 @@ import pytest
 pytest.importorskip("torch")
 
 from decodebench_b200 import _native as N  # noqa: E402
-from tests.test_paged_cpu import EDTYPE, ENULL, ESHAPE, append, attend, plan  # noqa: E402
+from tests.test_paged_cpu import EDTYPE, ENULL, ESHAPE, append, attend, plan, sample  # noqa: E402
 
 
 @pytest.mark.parametrize("dt,want", [
@@ -57,3 +57,11 @@ def test_page_plan_outputs_that_overlap(kw):
     if kw.get("used") == 0x9000 + 36:
         apart.update(slots=0x9000)
     assert plan(**apart) == ESHAPE
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=0x1000 + 792), dict(out=0x2000 - 8), dict(t=0x7000 + 12), dict(k=0x7000), dict(p=0x7000 + 8),
+    dict(mp=0x7000 - 4)])
+def test_sample_outputs_that_overlap(kw):
+    """2 rows of 100 fp32 logits; 16 bytes of tokens."""
+    assert sample(**{**dict(x=0x1000, u=0x2000, out=0x7000), **kw}) == ESHAPE
