@@ -47,15 +47,13 @@ def test_chunk_attention_outputs_that_overlap(kw):
 
 @pytest.mark.parametrize("kw", [
     dict(lens=0x1000), dict(lens=0x2000 + 4), dict(cu=0x1000 - 8), dict(table=0x3000 + 12), dict(table=0x1000 - 60),
-    dict(pos=0x8000), dict(slots=0x7000 + 16), dict(used=0x5000 + 8), dict(used=0x3000), dict(used=0x9000 + 36)])
+    dict(pos=0x8000), dict(slots=0x7000 + 16), dict(used=0x5000 + 4), dict(used=0x3000), dict(used=0x8000 + 36)])
 def test_page_plan_outputs_that_overlap(kw):
     """2 requests of 8 pages, 4 free pages, 5 tokens; seq_lens written over ctx_lens would be read by
     other blocks."""
     apart = dict(ctx=0x1000, new=0x2000, free=0x3000, table=0x4000, lens=0x5000, cu=0x6000, pos=0x7000,
-                 slots=0x8000, used=0x9000 if "used" not in kw else 0)
+                 slots=0x8000, used=0x9000)
     apart.update(kw)
-    if kw.get("used") == 0x9000 + 36:
-        apart.update(slots=0x9000)
     assert plan(**apart) == ESHAPE
 
 
