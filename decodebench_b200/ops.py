@@ -675,8 +675,9 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         # Not zero-filled and not kept: the caching allocator orders reuse by stream, and a
         # captured graph gets its own.
         workspace = torch.empty(nb, dtype=torch.uint8, device=dev)
-    elif workspace.dtype != torch.uint8 or workspace.device != dev or workspace.numel() < nb:
-        raise ValueError(f"workspace must be a uint8 tensor of >= {nb} bytes on {dev}")
+    elif (workspace.dtype != torch.uint8 or workspace.device != dev or workspace.numel() < nb or
+          not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of >= {nb} bytes on {dev}")
     _launch("dbk_chunk_attention", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             cu_seqlens.data_ptr(), seq_lens.data_ptr(), _ptr(page_table), o.data_ptr(), tokens,
             batch, hq, hkv, D, pages, page_size, max_pages, float(scale),

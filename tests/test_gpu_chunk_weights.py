@@ -131,3 +131,12 @@ def test_refuses_other_parts():
     for bad in (0, 3, None, "two"):
         with pytest.raises(ValueError, match="weight_parts"):
             ops.chunk_attention(q, k, v, cu, lens, page_table=table, weight_parts=bad)
+
+
+def test_refuses_a_workspace_whose_bytes_are_not_there():
+    """An expanded tensor has as many elements as asked for and one byte of memory."""
+    q, k, v, cu, lens, table = make([20], [3], 2, 1, 16, torch.bfloat16)
+    for bad in (torch.zeros(1, dtype=torch.uint8, device="cuda").expand(1 << 26),
+                torch.zeros(1 << 26, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.chunk_attention(q, k, v, cu, lens, page_table=table, workspace=bad)
