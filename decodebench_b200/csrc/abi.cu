@@ -225,7 +225,7 @@ extern "C" int dbk_take_device_error(void) {
   if (e != cudaSuccess) return (int)e;
   e = cudaMemcpyToSymbol(dbk::dbk_device_error, &zero, sizeof(int));
   if (e != cudaSuccess) return (int)e;
-  int w = 0;
+  int w = 0;                                  // of the file with a flag of its own
   if (int rc = dbk::chunk_take_error(&w)) return rc;
   return v ? v : w;
 }
@@ -260,7 +260,8 @@ __global__ void bounded_wait_probe_kernel(int which) {
 }  // namespace dbk
 
 extern "C" int dbk_test_bounded_wait(int which, void* stream) {
-  if (which != 0 && which != 1) return DBK_ESHAPE;
+  if (which < 0 || which > 3) return DBK_ESHAPE;
+  if (which >= 2) return dbk::chunk_test_bounded_wait(which - 2, static_cast<cudaStream_t>(stream));
   dbk::bounded_wait_probe_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(which);
   return (int)cudaGetLastError();
 }

@@ -1145,6 +1145,25 @@ int launch(ChunkArgs& a, const DeviceInfo& dev, cudaStream_t st) {
 
 }  // namespace
 
+namespace {
+// One warp and a barrier that nobody arrives at, by this file's two kinds of wait.
+__global__ void chunk_wait_probe_kernel(int branchless) {
+  __shared__ uint64_t bar;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (!branchless) (void)warp_wait(&bar, 0, kDevTimeoutEmpty);
+  else if (!poll_wait(&bar, 0, spin_limit()) && threadIdx.x == 0) record_error(kDevTimeoutMma);
+}
+}  // namespace
+
+int chunk_test_bounded_wait(int branchless, cudaStream_t stream) {
+  chunk_wait_probe_kernel<<<1, 32, 0, stream>>>(branchless);
+  return (int)cudaGetLastError();
+}
+
 int chunk_take_error(int* code) {
   const int zero = 0;
   cudaError_t e = cudaMemcpyFromSymbol(code, dbk_device_error, sizeof(int));

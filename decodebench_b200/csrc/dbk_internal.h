@@ -30,6 +30,7 @@ int allow_dynamic_smem(const void* kern, const DeviceInfo& dev, size_t smem);
 // budget: that file is built as a whole program (common.cuh).
 int chunk_take_error(int* code);
 int chunk_set_spin_limit(uint32_t polls);
+int chunk_test_bounded_wait(int branchless, cudaStream_t stream);
 
 struct PeerSet;   // comm.cuh
 // The peers of an open communicator, for kernels that fuse the all-gather

@@ -69,7 +69,10 @@ int dbk_set_spin_limit(uint32_t polls);
 /* Test hook (no counterpart in the reference): launches one CTA that runs the
  * library's bounded wait on an event that never happens -- which = 0: an
  * mbarrier nobody arrives at (records 1, "stage never filled"); which = 1: a
- * peer flag nobody raises (records 5, "peer signal missing"). The kernel gives
+ * peer flag nobody raises (records 5, "peer signal missing"); which = 2, 3: an
+ * mbarrier nobody arrives at, by the two kinds of wait of dbk_chunk_attention,
+ * which has a flag and a budget of its own behind the same calls (record 2,
+ * "stage never drained", and 3, "no tensor-core commit"). The kernel gives
  * up after the spin budget, records the code for dbk_take_device_error and
  * returns, leaving the context usable. */
 int dbk_test_bounded_wait(int which, void* stream);
