@@ -518,14 +518,17 @@ class PagePlan(NamedTuple):
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
+def _on(dev: torch.device, call, *args):
+    """``call(*args)`` with ``dev`` current."""
+    if _current_device() == dev.index:
+        return call(*args)
+    with torch.cuda.device(dev):
+        return call(*args)
+
+
 def _launch(fn: str, dev: torch.device, *args) -> None:
     """Calls ``fn(*args, stream)`` on ``dev``'s current stream, with ``dev`` current."""
-    call = getattr(N.load(), fn)
-    if _current_device() == dev.index:
-        status = call(*args, _stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = call(*args, _stream(dev))
+    status = _on(dev, getattr(N.load(), fn), *args, _stream(dev))
     if status != 0:
         raise N.DbkError(fn, status)
 
@@ -670,7 +673,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lib = N.load()
     some = min(tokens, 129)      # the size stops growing before that many tokens
     nb = _ws_bytes(("chunk", dev.index, some, hq, hkv),
-                   lambda: lib.dbk_chunk_attention_workspace_bytes(some, hq, hkv))
+                   lambda: _on(dev, lib.dbk_chunk_attention_workspace_bytes, some, hq, hkv))
     if workspace is None:
         # Not zero-filled and not kept: the caching allocator orders reuse by stream, and a
         # captured graph gets its own.
