@@ -77,7 +77,7 @@ struct ChunkArgs {
   const int32_t* cu;         // [batch + 1] first row of each sequence's new tokens
   const int32_t* lens;       // [batch] tokens in the cache, the new ones included
   const int32_t* pages;      // [batch, max_pages] or nullptr (contiguous)
-  const void *q, *k, *v;
+  const void* v;             // the cache's values
   void* out;
   float* part_o;             // [2 * grid][32][slot_rows][4]: column fours, rows, columns
   float2* part_ml;           // [2 * grid][slot_rows] (maximum in log2 units, sum)
@@ -1242,7 +1242,7 @@ extern "C" int dbk_chunk_attention(const void* q, const void* k_cache, const voi
   if (!aligned16(workspace)) return DBK_EALIGN;
 
   ChunkArgs a{};
-  a.q = q; a.k = k_cache; a.v = v_cache;
+  a.v = v_cache;
   a.cu = cu_seqlens; a.lens = seq_lens; a.pages = page_table; a.out = out;
   a.batch = batch; a.tokens = tokens; a.hq = n_q_heads; a.hkv = n_kv_heads;
   a.G = G; a.T = kRows / G;
