@@ -206,7 +206,7 @@ extern "C" const char* dbk_status_string(int s) {
   switch (s) {
     case DBK_OK: return "ok";
     case DBK_ENULL: return "a required pointer is NULL";
-    case DBK_ESHAPE: return "a size is outside the supported range";
+    case DBK_ESHAPE: return "a size is outside the supported range, or an output overlaps an input";
     case DBK_EALIGN: return "a pointer or row stride is not 16-byte aligned";
     case DBK_EWORKSPACE: return "workspace missing or too small";
     case DBK_EDTYPE: return "unknown dtype";

@@ -50,9 +50,10 @@ namespace dbk {
 namespace {
 
 // Threads of a CTA. Many rows (256 x 128,000 fp32: 265 us): small CTAs, three on an SM, whose phases
-// hide each other's barriers (four have 64 registers a thread, which spill: 273 us; five: 293). At
-// most one CTA per SM: larger ones, for a slice's passes are chains of dependent instructions (one
-// row of 128,000: 24 us with 512 threads; two to an SM, with 64 registers: 27).
+// hide each other's barriers (80 registers a thread, 16 to 104 bytes of them spilled; four have 64
+// and spill 88 to 428: 273 us; five: 293). At most one CTA per SM: larger ones, for a slice's passes are
+// chains of dependent instructions (one row of 128,000: 24 us with 512 threads; two to an SM, with
+// 64 registers: 27).
 constexpr int kManyThreads = 256, kManyCtas = 3, kFewThreads = 512, kMaxWarps = 32;
 constexpr int kBins = 256;
 constexpr float kFine = 14.f;       // log2 distances of the general path's first histogram

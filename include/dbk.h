@@ -36,7 +36,7 @@ typedef enum { DBK_F16 = 0, DBK_BF16 = 1 } dbk_dtype;
 /* Argument errors (negative). Positive values are cudaError_t. */
 #define DBK_OK 0
 #define DBK_ENULL (-1)        /* a required pointer is NULL                         */
-#define DBK_ESHAPE (-2)       /* a size is out of the supported range                */
+#define DBK_ESHAPE (-2)       /* a size is out of the supported range, or an output overlaps an input */
 #define DBK_EALIGN (-3)       /* a pointer or row is not 16-byte aligned             */
 #define DBK_EWORKSPACE (-4)   /* workspace missing or smaller than dbk_workspace_bytes */
 #define DBK_EDTYPE (-5)       /* unknown dtype                                        */
@@ -272,7 +272,8 @@ int dbk_gateup_swiglu_fp8(const void* x, const void* gamma, const void* Wg8, con
  *                       token get position 0 and slot -1; tokens behind the `tokens`-th are left out.
  *   used                int32 [1]: free pages the step needs (more than n_free: it lacked some)
  * Requests' token total and lengths stay below 2^31; batch <= 16384; outputs overlap neither
- * inputs nor one another (DBK_ESHAPE). Any later call may follow directly: the plan is complete before it starts. */
+ * inputs nor one another (DBK_ESHAPE). Any later call may follow directly: the plan is complete
+ * before it starts. */
 int dbk_page_plan(const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_pages,
                   int32_t* page_table, int32_t* seq_lens, int32_t* cu_seqlens,
                   int32_t* positions, int64_t* slots, int32_t* used, int batch, int n_free,

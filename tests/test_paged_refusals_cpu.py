@@ -63,3 +63,7 @@ def test_page_plan_outputs_that_overlap(kw):
 def test_sample_outputs_that_overlap(kw):
     """2 rows of 100 fp32 logits; 16 bytes of tokens."""
     assert sample(**{**dict(x=0x1000, u=0x2000, out=0x7000), **kw}) == ESHAPE
+
+
+def test_the_status_of_an_overlap_says_so():
+    assert "overlap" in N.status_string(ESHAPE)
