@@ -21,13 +21,15 @@
 // rounded once, to four digits); as one value it is 1.3 times that, and faster (below: "one part").
 //
 // What bounds it. A block of an item with two tiles is 2 x 3 x 128^3 products, 3,072 cycles of the
-// tensor core, and 2,048 of the exponential unit; it takes ~4,100 (one part: 2,048, ~3,000): the two
-// tiles' chains (S -> softmax -> PV -> next S) overlap but for their ends. One prompt of 16,384
-// tokens, 32 / 8 heads: 2.48 to 2.63 ms from one GPU to another (one part: 1.72 to 1.90), 1.25 to 1.33
-// PFLOP/s of issued products (a plain square library product under the same power limit: 1.68 in
-// bursts, 1.40 sustained). Few rows over a long cache are bound by HBM: 8 requests of one token at
-// 16,384, 64 / 8 heads: 102 us, 5.2 TB/s. Short calls pay ~9 us from launch to the first product (cold
-// code, lengths, cuts, first tiles) and ~4 for the join.
+// tensor core, and 2,048 of the exponential unit; it takes ~4,300 (tensor pipe active 71 % of the
+// cycles of a prompt of 8,192 tokens; one part: 2,048, ~3,400): the two tiles' chains (S -> softmax ->
+// PV -> next S) overlap but for their ends. One prompt of 16,384 tokens, 32 / 8 heads: 2.40 to 2.73 ms
+// from one GPU to another at 1,650 MHz under the power limit (one part: 1.72 to 2.06), 1.21 to 1.37
+// PFLOP/s of issued products (a plain square library product: 1.68 in bursts, 1.40 sustained). Few
+// rows over a long cache are bound by HBM: 8 requests of one token at 16,384, 64 / 8 heads: 103 us,
+// 5.2 TB/s. Short calls pay ~9 us from launch to the first product (cold code, lengths, cuts, first
+// tiles) and ~4 for the join; the pages' size makes no difference (24 ragged prompts in pages of
+// 16, 32, 64 and 128: 298 to 309 us).
 // Measured and not kept: a share of the exponentials by polynomial on the FMA pipe (1/8: +2 %,
 // 1/2: +13 %), two issuing threads (+18 %: the tiles fall into step), no row maximum but a bound
 // from the weights' sum (+12 %), S loaded from TMEM in two halves (+10 %).

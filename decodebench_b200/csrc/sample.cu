@@ -27,9 +27,10 @@
 // What bounds it. Many rows: dependent instructions (~120 a logit, all passes together; half of the
 // issue slots taken by 24 warps on an SM) and the barriers between passes. 256 rows of 128,000 fp32,
 // top-p: 265 us, 131 MB from HBM once, 0.49 TB/s, where a read alone takes 20 us. Few rows: a chain of
-// ~30 barriers and the latency of each pass (one row of 128,000: 24 us). Measured and not kept: the slice in registers over all passes
-// (unrolled, it misses the instruction cache: slower by half), 8-wide fp32 groups (8 % slower), a
-// larger share of shared memory (no change).
+// ~30 barriers and the latency of each pass (one row of 128,000: 24 us). The general path: 190 us for
+// one row of 300,001 with top-p, 199 for 8 of 262,208 with top-k and top-p. Measured and not kept: the
+// slice in registers over all passes (unrolled, it misses the instruction cache: slower by half),
+// 8-wide fp32 groups (8 % slower), a larger share of shared memory (no change).
 //
 // Rounding. The answer is an index, and a cut that falls on another side of a sum changes it,
 // so weights and sums are wider than 32-bit floats: common path, 30-bit weights (Exp2Table) as
