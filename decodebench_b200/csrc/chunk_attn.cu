@@ -23,8 +23,8 @@
 // What bounds it. A block of an item with two tiles is 2 x 3 x 128^3 products, 3,072 cycles of the
 // tensor core, and 2,048 of the exponential unit; it takes ~4,300 (tensor pipe active 71 % of the
 // cycles of a prompt of 8,192 tokens; one part: 2,048, ~3,400): the two tiles' chains (S -> softmax ->
-// PV -> next S) overlap but for their ends. One prompt of 16,384 tokens, 32 / 8 heads: 2.40 to 2.73 ms
-// from one GPU to another at 1,650 MHz under the power limit (one part: 1.72 to 2.06), 1.21 to 1.37
+// PV -> next S) overlap but for their ends. One prompt of 16,384 tokens, 32 / 8 heads: 2.40 to 2.77 ms
+// from call to call, around 1,650 MHz under the power limit (one part: 1.72 to 2.07), 1.19 to 1.37
 // PFLOP/s of issued products (a plain square library product: 1.68 in bursts, 1.40 sustained). Few
 // rows over a long cache are bound by HBM: 8 requests of one token at 16,384, 64 / 8 heads: 103 us,
 // 5.2 TB/s. Short calls pay ~9 us from launch to the first product (cold code, lengths, cuts, first
