@@ -833,8 +833,8 @@ __global__ void __launch_bounds__(NT, NT == kManyThreads ? kManyCtas : 1) sample
     cluster.sync();
     return;
   }
-  // To the general path: infinite logits, which share the draw; draws that may end among the weights this path
-  // drops (2^18 of less than 2^-46: 2^-28 of the largest).
+  // To the general path: infinite logits, which share the draw; draws that may end among the weights
+  // this path drops (2^18 of less than 2^-46: 2^-28 of the largest).
   if ((M == INFINITY || R.u < 0x1p-24f) && !greedy) {
     cluster.sync();
     general_row<T, NT>(a, R, M, *reinterpret_cast<SampleShared*>(dyn), dyn + sizeof(SampleShared) / sizeof(double));

@@ -639,7 +639,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``weight_parts``: the tensor cores get each softmax weight as the sum of two values of the
     cache's type, which leaves the result's own rounding as the only one of its size, or as one (1),
-    which adds half a step of the weights and takes about 0.7 of a prompt's time."""
+    which adds half a step of the weights and takes about three quarters of a prompt's time."""
     dev = (_cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens) if page_table is None else
            _cuda_device(q, k_cache, v_cache, cu_seqlens, seq_lens, page_table))
     _check_out(out, dev)
